@@ -364,6 +364,73 @@ int ani_scale_by_loss_f32(float* grads, long long n, const float* l2s, int n_mol
                           void* stream);
 
 /*
+ * Normalised layers and activations kept in 8 bits, for atomic networks whose layers are act(norm(A W + b)); no counterpart
+ * in the reference.  Rows are atoms in element order, acs_host counts them; gain_host, bias_host and the outputs named
+ * grad_*_host are HOST arrays of four device pointers, one per element (NULL where the element has no rows; the sums of an
+ * element without rows are written as zeros where a pointer is given).  1 <= width <= 4096.  Strides count values, are at
+ * least the width and need no alignment; rows that are 16-byte aligned are read faster.  Outputs are contiguous and written,
+ * not added to.  Nothing is allocated: the calls with sums over rows take a workspace of the stated size (one per call in
+ * flight; its content does not matter; size 0: NULL will do).  All sums are formed in a fixed order, in the type of the rows:
+ * results are bit-reproducible.
+ *
+ * Layer norm:  y = gain (x - mean) rstd + bias,  rstd = 1 / sqrt(variance + eps)  (variance: divided by the width).
+ */
+int ani_layer_norm_f32(const float* x, long long x_stride, const float* const* gain_host, const float* const* bias_host,
+                       int width, double eps, const int* acs_host, float* y, float* mean, float* rstd, void* stream);
+int ani_layer_norm_f64(const double* x, long long x_stride, const double* const* gain_host,
+                       const double* const* bias_host, int width, double eps, const int* acs_host, double* y, double* mean,
+                       double* rstd, void* stream);
+
+/* Its gradients; workspace: ani_layer_sums_workspace_bytes(width, acs_host, 2, sizeof a value). */
+int ani_layer_norm_grad_f32(const float* grad_y, long long grad_stride, const float* x, long long x_stride,
+                            const float* const* gain_host, const float* mean, const float* rstd, int width,
+                            const int* acs_host, float* grad_x, float* const* grad_gain_host, float* const* grad_bias_host,
+                            void* workspace, void* stream);
+int ani_layer_norm_grad_f64(const double* grad_y, long long grad_stride, const double* x, long long x_stride,
+                            const double* const* gain_host, const double* mean, const double* rstd, int width,
+                            const int* acs_host, double* grad_x, double* const* grad_gain_host,
+                            double* const* grad_bias_host, void* workspace, void* stream);
+size_t ani_layer_sums_workspace_bytes(int width, const int* acs_host, int sums, int value_bytes);
+
+/*
+ * Activation with an 8-bit checkpoint of its input:  a = act(z), or act(norm(z)) where gain_host and bias_host are given
+ * (both or neither).  `activation` as in ani_mlp_forward_f32.  The checkpoint is what the two calls below read:
+ *   codes  [n][ani_checkpoint_row_bytes(width)]   one byte a value (16-byte aligned; bytes behind the width are unspecified)
+ *   blocks [n][ani_checkpoint_blocks(width)][2]   base and step of every 128 columns (8-byte aligned)
+ *   mean, rstd [n]                                of z itself, with a norm only
+ * A code stands for base + code * step:  base = min, step = (max - min) * (1 / 255), code = rint((z - base) * (1 / step)),
+ * every operation rounded to float32; a block whose step is below 1e-30 has step 0, one that holds something that is not
+ * finite, or spans more than the largest float, has base NaN.  The value is off by half a step at most, but for rounding.
+ */
+int ani_checkpoint_row_bytes(int width);
+int ani_checkpoint_blocks(int width);
+int ani_checkpoint_activation_f32(const float* z, long long z_stride, const float* const* gain_host,
+                                  const float* const* bias_host, int width, double eps, int activation, const int* acs_host,
+                                  float* a, unsigned char* codes, float* blocks, float* mean, float* rstd, void* stream);
+
+/*
+ * Its backward pass from the checkpoint:  grad_z from grad_a, the column sums of grad_z per element (the gradient of the
+ * dense layer's bias, grad_sum_host) and with a norm those of its gain and bias.
+ * workspace: ani_layer_sums_workspace_bytes(width, acs_host, 3, 4).
+ */
+int ani_checkpoint_activation_grad_f32(const unsigned char* codes, const float* blocks, const float* mean, const float* rstd,
+                                       const float* grad_a, long long grad_stride, const float* const* gain_host,
+                                       const float* const* bias_host, int width, int activation, const int* acs_host,
+                                       float* grad_z, float* const* grad_sum_host, float* const* grad_gain_host,
+                                       float* const* grad_bias_host, void* workspace, void* stream);
+
+/*
+ * Weight gradient of the dense layer behind the activation:  grad_w[t] = sum over the rows of element t of
+ * act(...)^T grad_z,  [width][out_width], the activations recomputed from the checkpoint; 1 <= out_width <= 4096.
+ * workspace: ani_checkpoint_weight_grad_workspace_bytes(width, out_width, acs_host).
+ */
+int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* blocks, const float* mean, const float* rstd,
+                                   const float* const* gain_host, const float* const* bias_host, int width, int activation,
+                                   const float* grad_z, long long grad_stride, int out_width, const int* acs_host,
+                                   float* const* grad_w_host, void* workspace, void* stream);
+size_t ani_checkpoint_weight_grad_workspace_bytes(int width, int out_width, const int* acs_host);
+
+/*
  * AniCharge -- replaces the op of gpu_featurizer/ani_charges.cpp:45-56,58-113 (CPU, float and
  * double) and gpu_featurizer/ani_charges_gpu.cu:60-128 (GPU, float only).  Damped Coulomb
  * energy of every molecule,

@@ -18,7 +18,8 @@ CSRC = os.path.join(_HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include")
 SOURCES = ["ani_b200.cu"]
 HEADERS = ["ani_params.h", "ani_common.cuh", "ani_device_math.cuh", "ani_feeder.h", "ani_driver.h", "ani_mt19937.h", "ani_peer.cuh", "ani_sort.cuh", "ani_featurize.cuh", "ani_featurize_mol.cuh", "ani_featurize_large.cuh", "ani_featurize_round_passes.inl", "ani_grad.cuh", "ani_grad_mol.cuh", "ani_grad_large.cuh", "ani_grad_pair_pass.inl",
-           "ani_grad_inverse.cuh", "ani_tangent_mol.cuh", "ani_mlp.cuh", "ani_mlp_pipe.cuh", "ani_mlp_forward.cuh", "ani_mlp_backward.cuh", "ani_mlp_wgrad.cuh", "ani_mlp_small.cuh", "ani_mlp_chain.cuh", "ani_force_fit.cuh", "ani_launch.cuh", "ani_charge.cuh", "ani_optim.cuh", "ani_energy.cuh", "ani_host_pack.h"]
+           "ani_grad_inverse.cuh", "ani_tangent_mol.cuh", "ani_mlp.cuh", "ani_mlp_pipe.cuh", "ani_mlp_forward.cuh", "ani_mlp_backward.cuh", "ani_mlp_wgrad.cuh", "ani_mlp_small.cuh", "ani_mlp_chain.cuh", "ani_force_fit.cuh", "ani_launch.cuh", "ani_charge.cuh", "ani_optim.cuh", "ani_energy.cuh", "ani_host_pack.h",
+           "ani_norm.cuh", "ani_checkpoint.cuh", "ani_checkpoint_wgrad.cuh", "ani_layers.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -28,6 +29,7 @@ NVCC_FLAGS = [
 # the binding of the operators on torch tensors (csrc/torch_ops.cpp), an extension module of this package
 OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 OPS_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
+OPS_DEPENDS = [OPS_SOURCE, os.path.join(CSRC, "torch_layers.h")]
 
 _lock = threading.Lock()
 _lib = None
@@ -216,6 +218,17 @@ SIGNATURES = {
     "ani_charge_f64": (_i, [_vp] * 6 + [_i, _i, _vp, _vp]),
     "ani_charge_grad_f32": (_i, [_vp] * 6 + [_i, _i, _vp, _vp, _vp]),
     "ani_charge_grad_f64": (_i, [_vp] * 6 + [_i, _i, _vp, _vp, _vp]),
+    "ani_layer_norm_f32": (_i, [_vp, ctypes.c_longlong, _vp, _vp, _i, ctypes.c_double, c_int_p] + [_vp] * 4),
+    "ani_layer_norm_f64": (_i, [_vp, ctypes.c_longlong, _vp, _vp, _i, ctypes.c_double, c_int_p] + [_vp] * 4),
+    "ani_layer_norm_grad_f32": (_i, [_vp, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp, _vp, _vp, _i, c_int_p] + [_vp] * 5),
+    "ani_layer_norm_grad_f64": (_i, [_vp, ctypes.c_longlong, _vp, ctypes.c_longlong, _vp, _vp, _vp, _i, c_int_p] + [_vp] * 5),
+    "ani_layer_sums_workspace_bytes": (ctypes.c_size_t, [_i, c_int_p, _i, _i]),
+    "ani_checkpoint_row_bytes": (_i, [_i]),
+    "ani_checkpoint_blocks": (_i, [_i]),
+    "ani_checkpoint_activation_f32": (_i, [_vp, ctypes.c_longlong, _vp, _vp, _i, ctypes.c_double, _i, c_int_p] + [_vp] * 6),
+    "ani_checkpoint_activation_grad_f32": (_i, [_vp] * 5 + [ctypes.c_longlong, _vp, _vp, _i, _i, c_int_p] + [_vp] * 6),
+    "ani_checkpoint_weight_grad_f32": (_i, [_vp] * 6 + [_i, _i, _vp, ctypes.c_longlong, _i, c_int_p] + [_vp] * 3),
+    "ani_checkpoint_weight_grad_workspace_bytes": (ctypes.c_size_t, [_i, _i, c_int_p]),
     "ani_mlp_forward_f32": (_i, [ctypes.POINTER(MlpArgs), c_int_p, _i, _i, _vp]),
 }
 
@@ -256,7 +269,7 @@ def build_ops(force: bool = False) -> str:
 
     from torch.utils import cpp_extension
     with _lock:
-        if not force and os.path.exists(OPS_PATH) and os.path.getmtime(OPS_PATH) >= os.path.getmtime(OPS_SOURCE):
+        if not force and os.path.exists(OPS_PATH) and os.path.getmtime(OPS_PATH) >= max(os.path.getmtime(f) for f in OPS_DEPENDS):
             return OPS_PATH
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-pthread", "-shared", "-DTORCH_EXTENSION_NAME=_torch_ops", OPS_SOURCE, "-o", OPS_PATH]
         import numpy
@@ -280,6 +293,11 @@ def torch_ops():
         from . import _torch_ops as mod
         mod.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
             "ani_sort", "ani_featurize_f32", "ani_featurize_f64", "ani_featurize_grad_f32", "ani_featurize_grad_f64")))
+        mod.bind_layers([ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
+            "ani_layer_norm_f32", "ani_layer_norm_f64", "ani_layer_norm_grad_f32", "ani_layer_norm_grad_f64",
+            "ani_layer_sums_workspace_bytes", "ani_checkpoint_activation_f32", "ani_checkpoint_activation_grad_f32",
+            "ani_checkpoint_weight_grad_f32", "ani_checkpoint_weight_grad_workspace_bytes", "ani_checkpoint_row_bytes",
+            "ani_checkpoint_blocks")])
         _ops = mod
     return _ops
 

@@ -1794,3 +1794,5 @@ int ani_force_fit_pass_beside_f32(const ani_force_fit_args* f, void* side_stream
 }
 
 }  // extern "C"
+
+#include "ani_layers.h"

@@ -1,0 +1,243 @@
+// Activations of a layer whose input is kept in 8 bits for the backward pass.
+//
+// Forward, row by row (z: what the dense layer left; with a gain, u = gain (z - mean) rstd + bias, else u = z):
+//   a = act(u);  codes: of every block of 128 columns  base = min z, step = (max z - min z) / 255,
+//   code = rint((z - base) / step) in 0 .. 255, one byte;  mean and rstd are those of z itself.
+// Backward, from codes alone:  z~ = base + code step (|z~ - z| <= step / 2),  u~ from z~ as u from z,
+//   du = da act'(u~);  without gain dz = du, with it dz as in the layer norm's backward pass with xhat~ = (z~ - mean) rstd;
+//   column sums of dz (the gradient of the dense layer's bias) and with a gain of du xhat~ and du.
+// The codes are defined by float32 operations, each rounded once, so that they do not depend on who computes them:
+//   step = (max - min) * (1 / 255),  code = rint((z - base) * (1 / step)),
+// a block whose step is below 1e-30 is its base (step 0).  Counting from the minimum, not from the middle or from zero,
+// keeps z - base exact where it matters: a block far from zero still has all of its 256 steps.  A block that holds something
+// that is not finite, or that spans more than the largest float, has base NaN: its gradients are NaN and not wrong.
+//
+// One byte a value and 8 bytes a block (6 %) instead of the 8 bytes a value that z and a, or a and its derivative, take.
+#pragma once
+
+#include "ani_mlp.cuh"
+#include "ani_norm.cuh"
+
+namespace ani {
+
+constexpr int kCheckpointBlock = 128;
+__host__ __device__ __forceinline__ int checkpoint_row_bytes(int width) { return (width + 15) & ~15; }
+__host__ __device__ __forceinline__ int checkpoint_blocks(int width) { return (width + kCheckpointBlock - 1) / kCheckpointBlock; }
+
+__device__ __forceinline__ float act_value(int act, float u)
+{
+    if (act == kActCelu) return mlp_activation<kActCelu>(u);
+    if (act == kActGaussian) return mlp_activation<kActGaussian>(u);
+    if (act == kActNormal) return mlp_activation<kActNormal>(u);
+    return mlp_activation<kActSoftplus>(u);
+}
+__device__ __forceinline__ float act_derivative(int act, float u)
+{
+    if (act == kActCelu) return u >= 0.0f ? 1.0f : expf(u * 10.0f);
+    if (act == kActGaussian) return -2.0f * u * expf(-u * u);
+    if (act == kActNormal) return -u * expf(-0.5f * u * u);
+    return 1.0f / (1.0f + expf(-u));
+}
+
+// Smaller / larger of two values, NaN if one of them is.
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+struct CheckpointParams {
+    const float* z;
+    long long z_stride;
+    const float* gain[kTypes];
+    const float* bias[kTypes];
+    float* a;
+    unsigned char* codes;      // [n][checkpoint_row_bytes]
+    float2* blocks;            // [n][checkpoint_blocks]: base, step
+    float *mean, *rstd;
+    RowGroups groups;
+    int width, vec, act;
+    float inv_w, eps;
+};
+
+template <int TEAM, int NV, bool NORM>
+__global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(const __grid_constant__ CheckpointParams p)
+{
+    __shared__ float scratch[kNormThreads / kWarp];
+    constexpr int teams = kNormThreads / TEAM;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
+    const int row_bytes = checkpoint_row_bytes(w), row_blocks = checkpoint_blocks(w);
+    const long long n = p.groups.start[kTypes];
+    pdl_wait();
+    pdl_trigger();
+    for (long long first = (long long)blockIdx.x * teams; first < n; first += (long long)gridDim.x * teams) {
+        const bool live = first + team < n;
+        const long long row = live ? first + team : first;
+        float z[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+            load_columns(p.z + row * p.z_stride, 4 * (lane + k * TEAM), w, p.vec, z[k]);
+        float mean = 0.0f, rstd = 1.0f;
+        if (NORM) row_statistics<TEAM, NV>(z, lane, w, p.inv_w, p.eps, scratch, &mean, &rstd);
+        const int e = element_of_row(p.groups, row);
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            float low = __int_as_float(0x7f800000), high = -low;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (col + i < w) {
+                    low = min_nan(low, z[k][i]);
+                    high = max_nan(high, z[k][i]);
+                }
+#pragma unroll
+            for (int o = (TEAM < kWarp ? TEAM : kWarp) / 2; o > 0; o >>= 1) {
+                low = min_nan(low, __shfl_xor_sync(kFull, low, o));
+                high = max_nan(high, __shfl_xor_sync(kFull, high, o));
+            }
+            if (!live || col >= w) continue;
+            const float spread = __fsub_rn(high, low);
+            float step = __fmul_rn(spread, 1.0f / 255.0f);
+            const bool finite = spread < __int_as_float(0x7f800000), some = finite && step >= 1e-30f;
+            const float inv = some ? __frcp_rn(step) : 0.0f;
+            step = some ? step : 0.0f;
+            unsigned code = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float q = some && col + i < w ? fminf(rintf(__fmul_rn(__fsub_rn(z[k][i], low), inv)), 255.0f) : 0.0f;
+                code |= (unsigned)q << (8 * i);
+            }
+            *reinterpret_cast<unsigned*>(p.codes + row * row_bytes + col) = code;
+            if (col % kCheckpointBlock == 0)
+                p.blocks[row * row_blocks + col / kCheckpointBlock] = make_float2(finite ? low : __int_as_float(0x7fffffff), step);
+            float g[4], h[4];
+            if (NORM) {
+                load_columns(p.gain[e], col, w, p.vec, g);
+                load_columns(p.bias[e], col, w, p.vec, h);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[k][i] = act_value(p.act, NORM ? (z[k][i] - mean) * rstd * g[i] + h[i] : z[k][i]);
+            store_columns(p.a + row * w, col, w, p.vec, z[k]);
+        }
+        if (NORM && live && lane == 0) {
+            p.mean[row] = mean;
+            p.rstd[row] = rstd;
+        }
+    }
+}
+
+struct CheckpointGradParams {
+    const unsigned char* codes;
+    const float2* blocks;
+    const float *mean, *rstd;
+    const float* grad_a;
+    long long grad_stride;
+    const float* gain[kTypes];
+    const float* bias[kTypes];
+    float* grad_z;
+    ColumnSums<float, 3> sums;      // of dz, and with a gain of its gradient and the bias'
+    RowRanges ranges;
+    int width, vec, act;
+    float inv_w;
+};
+
+// The four values at column col that the codes of a row stand for.
+__device__ __forceinline__ void load_codes(const unsigned char* codes, const float2* blocks, int col, int w, float* z)
+{
+    const unsigned code = col < w ? *reinterpret_cast<const unsigned*>(codes + col) : 0u;
+    const float2 b = col < w ? blocks[col / kCheckpointBlock] : make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) z[i] = fmaf((float)((code >> (8 * i)) & 255u), b.y, b.x);
+}
+
+template <int TEAM, int NV, bool NORM>
+__global__ void __launch_bounds__(kNormThreads) checkpoint_activation_grad_kernel(const __grid_constant__ CheckpointGradParams p)
+{
+    constexpr int Q = NORM ? 3 : 1;
+    __shared__ float scratch[2 * kNormThreads / kWarp];
+    __shared__ alignas(16) float tile[TEAM == kNormThreads ? 4 : kNormThreads * NV * 4];
+    constexpr int teams = kNormThreads / TEAM;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
+    const int row_bytes = checkpoint_row_bytes(w), row_blocks = checkpoint_blocks(w);
+    pdl_wait();
+    pdl_trigger();
+    zero_sums_without_rows(p.sums, p.ranges, w);
+    if ((int)blockIdx.x >= p.ranges.range_start[kTypes]) return;      // no rows at all: one CTA, for the zeros
+    const RowRange range = range_of_cta(p.ranges, blockIdx.x);
+    float gain[NV][4], bias[NV][4], sums[Q][NV][4];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        if (NORM) {
+            load_columns(p.gain[range.element], 4 * (lane + k * TEAM), w, p.vec, gain[k]);
+            load_columns(p.bias[range.element], 4 * (lane + k * TEAM), w, p.vec, bias[k]);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sums[q][k][i] = 0.0f;
+    }
+    for (long long first = range.first; first < range.end; first += teams) {
+        const bool live = first + team < range.end;
+        const long long row = live ? first + team : first;
+        float kept[NV][4], up[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            load_codes(p.codes + row * row_bytes, p.blocks + row * row_blocks, col, live ? w : 0, kept[k]);
+            load_columns(p.grad_a + row * p.grad_stride, col, live ? w : 0, p.vec, up[k]);
+        }
+        if constexpr (NORM) {
+            const float mean = p.mean[row], rstd = p.rstd[row];
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int col = 4 * (lane + k * TEAM);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool in = live && col + i < w;
+                    const float xhat = in ? (kept[k][i] - mean) * rstd : 0.0f;
+                    const float du = in ? up[k][i] * act_derivative(p.act, xhat * gain[k][i] + bias[k][i]) : 0.0f;
+                    kept[k][i] = xhat;
+                    sums[Q - 2][k][i] += du * xhat;
+                    sums[Q - 1][k][i] += du;
+                    up[k][i] = du * gain[k][i];
+                    sum[0] += up[k][i];
+                    sum[1] += up[k][i] * xhat;
+                }
+            }
+            team_sum<TEAM, 2>(sum, scratch);
+            sum[0] *= p.inv_w;
+            sum[1] *= p.inv_w;
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) up[k][i] = rstd * (up[k][i] - sum[0] - kept[k][i] * sum[1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) up[k][i] *= act_derivative(p.act, kept[k][i]);
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            if (col >= w) break;
+#pragma unroll
+            for (int i = 0; i < 4; i++) sums[0][k][i] += up[k][i];
+            store_columns(p.grad_z + row * w, col, w, p.vec, up[k]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+        store_column_sums<TEAM, NV>(sums[q], tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, q, w), w);
+}
+
+}  // namespace ani

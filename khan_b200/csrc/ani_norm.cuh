@@ -1,0 +1,332 @@
+// Layer norm over the rows of the atomic networks, forward and backward, and the pieces that the kernels of activation
+// checkpoints share with it (ani_checkpoint.cuh).
+//
+// Rows are atoms in element order (start[t] .. start[t + 1] of element t), every element has its own gain and bias:
+//   mean = sum x / w,  rstd = 1 / sqrt(sum (x - mean)^2 / w + eps),  xhat = (x - mean) rstd,  y = gain xhat + bias;
+//   g = gain dy:  dx = rstd (g - sum g / w - xhat sum(g xhat) / w),  dgain = sum over rows dy xhat,  dbias = sum over rows dy.
+//
+// A row belongs to a TEAM of threads (8, 16 or 32 lanes of a warp, or a CTA of 256), which keeps it in registers: thread l
+// holds the NV groups of four consecutive columns 4 (l + k TEAM), so that the row is read once and the variance is the
+// two-pass one (a mean far from zero costs nothing).  Columns are four to a thread whether or not the rows are 16-byte
+// aligned; only the load instruction differs.  All sums are held in the type of the rows: 32 bits for float.
+//
+// Sums over rows: a CTA takes a contiguous range of rows of ONE element, its teams add up in registers, the CTA adds its
+// teams in order through shared memory and writes one partial row; a second launch adds the partial rows in order.  No
+// atomics: results do not change from run to run.  An element with one range is written by the first launch, and when that
+// holds for all of them there is no second one.
+#pragma once
+
+#include "ani_common.cuh"
+#include "ani_launch.cuh"
+
+namespace ani {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormMaxWidth = 4096;
+constexpr int kNormSms = 148;      // of a B200; the plans below only have to be good, not exact
+
+struct RowGroups {
+    long long start[kTypes + 1];   // rows of element t: start[t] .. start[t + 1]
+};
+// Ranges of rows, one per CTA, each of one element.
+struct RowRanges {
+    RowGroups groups;
+    long long rows;                // rows per range
+    int range_start[kTypes + 1];   // prefix of ceil(rows of the element / rows)
+};
+
+__device__ __forceinline__ int element_of_row(const RowGroups& g, long long row)
+{
+    return (row >= g.start[1] ? 1 : 0) + (row >= g.start[2] ? 1 : 0) + (row >= g.start[3] ? 1 : 0);
+}
+struct RowRange {
+    int element;
+    long long first, end;
+};
+__device__ __forceinline__ RowRange range_of_cta(const RowRanges& r, int cta)
+{
+    RowRange out;
+    out.element = 0;
+#pragma unroll
+    for (int t = 1; t < kTypes; t++) out.element += cta >= r.range_start[t] ? 1 : 0;
+    out.first = r.groups.start[out.element] + (long long)(cta - r.range_start[out.element]) * r.rows;
+    out.end = min(out.first + r.rows, r.groups.start[out.element + 1]);
+    return out;
+}
+
+// Four consecutive columns of a row; columns >= w read as zero and are not written.
+template <typename T> __device__ __forceinline__ void load_columns(const T* row, int col, int w, bool vec, T* v)
+{
+    if (vec && col + 4 <= w) {
+        load4(row + col, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = col + i < w ? row[col + i] : T(0);
+    }
+}
+__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store4(double* p, const double* v)
+{
+    *reinterpret_cast<double2*>(p) = make_double2(v[0], v[1]);
+    *reinterpret_cast<double2*>(p + 2) = make_double2(v[2], v[3]);
+}
+template <typename T> __device__ __forceinline__ void store_columns(T* row, int col, int w, bool vec, const T* v)
+{
+    if (vec && col + 4 <= w) {
+        store4(row + col, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (col + i < w) row[col + i] = v[i];
+    }
+}
+
+// Sums over a team, the same value in all of its threads.  Every thread of the CTA takes part.
+template <int TEAM, int N, typename T> __device__ __forceinline__ void team_sum(T* v, T* scratch)
+{
+#pragma unroll
+    for (int o = (TEAM < kWarp ? TEAM : kWarp) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(kFull, v[i], o);
+    if (TEAM > kWarp) {
+        __syncthreads();      // the values of the sum before have been read
+        if (lane_id() == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) scratch[warp_id() * N + i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            T s = T(0);
+#pragma unroll
+            for (int k = 0; k < TEAM / kWarp; k++) s += scratch[k * N + i];
+            v[i] = s;
+        }
+    }
+}
+
+__device__ __forceinline__ float rsqrt_full(float v) { return 1.0f / sqrtf(v); }
+__device__ __forceinline__ double rsqrt_full(double v) { return 1.0 / sqrt(v); }
+
+// mean and 1 / sqrt(variance + eps) of the row that the team holds in x.
+template <int TEAM, int NV, typename T>
+__device__ __forceinline__ void row_statistics(const T (*x)[4], int lane, int w, T inv_w, T eps, T* scratch, T* mean, T* rstd)
+{
+    T s = T(0);
+#pragma unroll
+    for (int k = 0; k < NV; k++) s += (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+    team_sum<TEAM, 1>(&s, scratch);
+    const T m = s * inv_w;
+    T q = T(0);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int col = 4 * (lane + k * TEAM);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const T d = col + i < w ? x[k][i] - m : T(0);
+            q += d * d;
+        }
+    }
+    team_sum<TEAM, 1>(&q, scratch);
+    *mean = m;
+    *rstd = rsqrt_full(q * inv_w + eps);
+}
+
+// The sums over the rows of a CTA's range, from the sums of its teams: added in the order of the teams and written to
+// out[0 .. w).  Every thread of the CTA takes part.
+template <int TEAM, int NV, typename T>
+__device__ __forceinline__ void store_column_sums(const T (*v)[4], T* tile, T* out, int w)
+{
+    constexpr int teams = kNormThreads / TEAM;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    if (TEAM == kNormThreads) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) store_columns(out, 4 * (lane + k * TEAM), w, false, v[k]);
+        return;
+    }
+    __syncthreads();      // the tile of the sums before has been read
+#pragma unroll
+    for (int k = 0; k < NV; k++) store4(tile + (size_t)team * (TEAM * NV * 4) + 4 * (lane + k * TEAM), v[k]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < w; c += kNormThreads) {
+        T s = T(0);
+#pragma unroll
+        for (int t = 0; t < teams; t++) s += tile[t * (TEAM * NV * 4) + c];
+        out[c] = s;
+    }
+}
+
+// What the launches with sums over rows write: Q sums per element, each [width].
+template <typename T, int Q> struct ColumnSums {
+    T* out[Q][kTypes];     // null: not wanted
+    T* partial;            // [ranges][Q][width]
+};
+template <typename T, int Q>
+__device__ __forceinline__ T* column_sums_place(const ColumnSums<T, Q>& s, const RowRanges& r, int element, int cta, int q, int w)
+{
+    return r.range_start[element + 1] - r.range_start[element] == 1 ? s.out[q][element] : s.partial + ((size_t)cta * Q + q) * w;
+}
+// Sums of an element without rows are zero: written by the first CTA of the first launch.
+template <typename T, int Q>
+__device__ __forceinline__ void zero_sums_without_rows(const ColumnSums<T, Q>& s, const RowRanges& r, int w)
+{
+    if (blockIdx.x) return;
+#pragma unroll
+    for (int t = 0; t < kTypes; t++)
+        if (r.range_start[t] == r.range_start[t + 1])
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (s.out[q][t])
+                    for (int c = threadIdx.x; c < w; c += kNormThreads) s.out[q][t][c] = T(0);
+}
+
+constexpr int kSumColumns = 32, kSumParts = 8;
+template <typename T, int Q>
+__global__ void __launch_bounds__(kSumColumns* kSumParts) column_sums_kernel(const ColumnSums<T, Q> s, const RowRanges r, int w)
+{
+    __shared__ T part[kSumParts][kSumColumns];
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.y / Q, q = blockIdx.y % Q, c = blockIdx.x * kSumColumns + threadIdx.x;
+    const int first = r.range_start[t], n = r.range_start[t + 1] - first;
+    if (n <= 1 || !s.out[q][t]) return;      // written by the first launch, or not wanted
+    T sum = T(0);
+    if (c < w)
+        for (int k = threadIdx.y; k < n; k += kSumParts) sum += s.partial[((size_t)(first + k) * Q + q) * w + c];
+    part[threadIdx.y][threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < w) {
+        sum = part[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kSumParts; k++) sum += part[k][threadIdx.x];
+        s.out[q][t][c] = sum;
+    }
+}
+
+// ------------------------------------------------------------------ layer norm
+template <typename T> struct LayerNormParams {
+    const T* x;
+    long long x_stride;
+    const T* gain[kTypes];
+    const T* bias[kTypes];
+    T *y, *mean, *rstd;
+    RowGroups groups;
+    int width, vec;
+    T inv_w, eps;
+};
+
+template <typename T, int TEAM, int NV>
+__global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const __grid_constant__ LayerNormParams<T> p)
+{
+    __shared__ T scratch[kNormThreads / kWarp];
+    constexpr int teams = kNormThreads / TEAM;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const long long n = p.groups.start[kTypes];
+    pdl_wait();
+    pdl_trigger();
+    for (long long base = (long long)blockIdx.x * teams; base < n; base += (long long)gridDim.x * teams) {
+        const long long row = base + team;
+        const bool live = row < n;
+        T x[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+            load_columns(p.x + (live ? row : 0) * p.x_stride, 4 * (lane + k * TEAM), live ? p.width : 0, p.vec, x[k]);
+        T mean, rstd;
+        row_statistics<TEAM, NV>(x, lane, p.width, p.inv_w, p.eps, scratch, &mean, &rstd);
+        if (!live) continue;      // the teams of a CTA of 256 are one, and live
+        const int e = element_of_row(p.groups, row);
+        const T *gain = p.gain[e], *bias = p.bias[e];
+        T* y = p.y + row * p.width;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            if (col >= p.width) break;
+            T g[4], h[4];
+            load_columns(gain, col, p.width, p.vec, g);
+            load_columns(bias, col, p.width, p.vec, h);
+#pragma unroll
+            for (int i = 0; i < 4; i++) g[i] = (x[k][i] - mean) * rstd * g[i] + h[i];
+            store_columns(y, col, p.width, p.vec, g);
+        }
+        if (lane == 0) {
+            p.mean[row] = mean;
+            p.rstd[row] = rstd;
+        }
+    }
+}
+
+template <typename T> struct LayerNormGradParams {
+    const T* grad_y;
+    long long grad_stride;
+    const T* x;
+    long long x_stride;
+    const T* gain[kTypes];
+    const T *mean, *rstd;
+    T* grad_x;
+    ColumnSums<T, 2> sums;      // gain, bias
+    RowRanges ranges;
+    int width, vec;
+    T inv_w;
+};
+
+template <typename T, int TEAM, int NV>
+__global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __grid_constant__ LayerNormGradParams<T> p)
+{
+    __shared__ T scratch[2 * kNormThreads / kWarp];
+    __shared__ alignas(16) T tile[TEAM == kNormThreads ? 4 : kNormThreads * NV * 4];
+    constexpr int teams = kNormThreads / TEAM;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
+    pdl_wait();
+    pdl_trigger();
+    zero_sums_without_rows(p.sums, p.ranges, w);
+    if ((int)blockIdx.x >= p.ranges.range_start[kTypes]) return;      // no rows at all: one CTA, for the zeros
+    const RowRange range = range_of_cta(p.ranges, blockIdx.x);
+    T gain[NV][4], dgain[NV][4], dbias[NV][4];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        load_columns(p.gain[range.element], 4 * (lane + k * TEAM), w, p.vec, gain[k]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) dgain[k][i] = dbias[k][i] = T(0);
+    }
+    for (long long base = range.first; base < range.end; base += teams) {
+        const bool live = base + team < range.end;
+        const long long row = live ? base + team : base;
+        T xhat[NV][4], up[NV][4];
+        const T mean = p.mean[row], rstd = p.rstd[row];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            load_columns(p.x + row * p.x_stride, col, live ? w : 0, p.vec, xhat[k]);
+            load_columns(p.grad_y + row * p.grad_stride, col, live ? w : 0, p.vec, up[k]);
+        }
+        T sum[2] = {T(0), T(0)};
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                xhat[k][i] = live && col + i < w ? (xhat[k][i] - mean) * rstd : T(0);
+                dgain[k][i] += up[k][i] * xhat[k][i];
+                dbias[k][i] += up[k][i];
+                up[k][i] *= gain[k][i];
+                sum[0] += up[k][i];
+                sum[1] += up[k][i] * xhat[k][i];
+            }
+        }
+        team_sum<TEAM, 2>(sum, scratch);
+        if (!live) continue;
+        sum[0] *= p.inv_w;
+        sum[1] *= p.inv_w;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            if (col >= w) break;
+#pragma unroll
+            for (int i = 0; i < 4; i++) up[k][i] = rstd * (up[k][i] - sum[0] - xhat[k][i] * sum[1]);
+            store_columns(p.grad_x + row * w, col, w, p.vec, up[k]);
+        }
+    }
+    store_column_sums<TEAM, NV>(dgain, tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, 0, w), w);
+    store_column_sums<TEAM, NV>(dbias, tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, 1, w), w);
+}
+
+}  // namespace ani

@@ -13,6 +13,8 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <pybind11/stl.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #define NPY_NO_DEPRECATED_API NPY_1_20_API_VERSION
@@ -20,6 +22,7 @@
 
 #include <stdint.h>
 
+#include <algorithm>
 #include <vector>
 
 namespace py = pybind11;
@@ -217,6 +220,8 @@ py::list split_rows(const py::object& rows, const py::object& cuts)
 
 }  // namespace
 
+#include "torch_layers.h"
+
 PYBIND11_MODULE(_torch_ops, m)
 {
     if (_import_array() < 0) throw py::error_already_set();
@@ -226,4 +231,10 @@ PYBIND11_MODULE(_torch_ops, m)
     m.def("featurize", &featurize);
     m.def("featurize_into", &featurize_into);
     m.def("featurize_grad", &featurize_grad);
+    m.def("bind_layers", &bind_layers);
+    m.def("layer_norm", &layer_norm);
+    m.def("layer_norm_grad", &layer_norm_grad);
+    m.def("checkpoint_activation", &checkpoint_activation);
+    m.def("checkpoint_activation_grad", &checkpoint_activation_grad);
+    m.def("checkpoint_weight_grad", &checkpoint_weight_grad);
 }

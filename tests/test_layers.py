@@ -1,0 +1,126 @@
+"""Normalised layers and activation checkpoints: what can be checked without a GPU (argument checks of the C entry points,
+refusals of the Python ones, the reference implementation of the GPU tests)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import layer_reference as ref
+from khan_b200 import _lib, layer_mod
+
+P = ctypes.c_void_p
+
+
+@pytest.fixture(scope="module")
+def handle():
+    _lib.build()
+    return _lib.lib()
+
+
+def four(*addresses):
+    return (ctypes.c_void_p * 4)(*(list(addresses) + [None] * (4 - len(addresses))))
+
+
+def test_sizes(handle):
+    assert [handle.ani_checkpoint_row_bytes(w) for w in (1, 16, 17, 128, 4096)] == [16, 16, 32, 128, 4096]
+    assert [handle.ani_checkpoint_blocks(w) for w in (1, 128, 129, 4096)] == [1, 1, 2, 32]
+    assert handle.ani_checkpoint_row_bytes(0) == handle.ani_checkpoint_blocks(4097) == -2
+    one, many = (ctypes.c_int * 4)(3, 0, 0, 2), (ctypes.c_int * 4)(100000, 0, 50000, 1)
+    assert handle.ani_layer_sums_workspace_bytes(128, one, 3, 4) == 0
+    small, large = (handle.ani_layer_sums_workspace_bytes(128, many, 3, s) for s in (4, 8))
+    assert small > 0 and large == 2 * small and small % (3 * 128 * 4) == 0
+    assert handle.ani_checkpoint_weight_grad_workspace_bytes(128, 64, one) == 0
+    assert handle.ani_checkpoint_weight_grad_workspace_bytes(128, 64, many) % (128 * 64 * 4) == 0
+    assert handle.ani_layer_sums_workspace_bytes(0, many, 3, 4) == handle.ani_checkpoint_weight_grad_workspace_bytes(1, 5000, many) == 0
+
+
+def test_layer_norm_checks_need_no_gpu(handle):
+    acs, bad, none = (ctypes.c_int * 4)(5, 0, 0, 2), (ctypes.c_int * 4)(5, -1, 0, 0), (ctypes.c_int * 4)()
+    v, x, y = four(0x10000, None, None, 0x20000), 0x30000, 0x40000
+    for fwd, grad in ((handle.ani_layer_norm_f32, handle.ani_layer_norm_grad_f32), (handle.ani_layer_norm_f64, handle.ani_layer_norm_grad_f64)):
+        assert fwd(None, 128, None, None, 128, 1e-5, none, None, None, None, None) == 0
+        assert fwd(x, 128, v, v, 128, 1e-5, None, y, y, y, None) == -1
+        assert fwd(None, 128, v, v, 128, 1e-5, acs, y, y, y, None) == fwd(x, 128, None, v, 128, 1e-5, acs, y, y, y, None) == -1
+        assert fwd(x, 128, four(0x10000), v, 128, 1e-5, acs, y, y, y, None) == fwd(x, 128, v, v, 128, 1e-5, acs, y, None, y, None) == -1
+        for width, stride, eps, counts in ((0, 128, 1e-5, acs), (4097, 5000, 1e-5, acs), (128, 127, 1e-5, acs), (128, 128, -1.0, acs),
+                                           (128, 128, float("nan"), acs), (128, 128, float("inf"), acs), (128, 128, 1e-5, bad)):
+            assert fwd(x, stride, v, v, width, eps, counts, y, y, y, None) == -2
+        assert grad(x, 127, x, 128, v, x, x, 128, acs, y, v, v, None, None) == grad(x, 128, x, 127, v, x, x, 128, acs, y, v, v, None, None) == -2
+        assert grad(x, 128, x, 128, v, x, x, 128, acs, y, None, v, None, None) == grad(x, 128, x, 128, v, x, x, 128, acs, None, v, v, None, None) == -1
+        # many rows need a workspace
+        assert grad(x, 128, x, 128, four(x), x, x, 128, (ctypes.c_int * 4)(100000), y, four(y), four(y), None, None) == -1
+
+
+def test_checkpoint_checks_need_no_gpu(handle):
+    acs, none, many = (ctypes.c_int * 4)(5), (ctypes.c_int * 4)(), (ctypes.c_int * 4)(100000)
+    v, x = four(0x10000), 0x30000
+    fwd, grad, wgrad = handle.ani_checkpoint_activation_f32, handle.ani_checkpoint_activation_grad_f32, handle.ani_checkpoint_weight_grad_f32
+    assert fwd(None, 64, None, None, 64, 0.0, 0, none, None, None, None, None, None, None) == 0
+    for act in (-1, 4):
+        assert fwd(x, 64, None, None, 64, 0.0, act, acs, x, x, x, None, None, None) == -2
+        assert grad(x, x, None, None, x, 64, None, None, 64, act, acs, x, v, None, None, None, None) == -2
+        assert wgrad(x, x, None, None, None, None, 64, act, x, 8, 8, acs, v, None, None) == -2
+    assert fwd(x, 63, None, None, 64, 0.0, 0, acs, x, x, x, None, None, None) == -2
+    assert fwd(x, 64, v, v, 64, -1.0, 0, acs, x, x, x, x, x, None) == -2
+    # a gain without a bias, a norm without a place for the statistics, codes and blocks that are not aligned
+    assert fwd(x, 64, v, None, 64, 0.0, 0, acs, x, x, x, x, x, None) == fwd(x, 64, v, v, 64, 0.0, 0, acs, x, x, x, None, x, None) == -1
+    assert fwd(x, 64, None, None, 64, 0.0, 0, acs, x, x + 8, x, None, None, None) == fwd(x, 64, None, None, 64, 0.0, 0, acs, x, x, x + 4, None, None, None) == -9
+    assert grad(x, x, None, None, x, 63, None, None, 64, 0, acs, x, v, None, None, None, None) == -2
+    assert grad(x, x, None, None, x, 64, None, None, 64, 0, acs, x, None, None, None, None, None) == -1
+    assert grad(x, x, x, x, x, 64, v, v, 64, 0, acs, x, v, v, None, None, None) == grad(x, x, None, x, x, 64, v, v, 64, 0, acs, x, v, v, v, None, None) == -1
+    assert grad(x + 1, x, None, None, x, 64, None, None, 64, 0, acs, x, v, None, None, None, None) == -9
+    assert grad(x, x, None, None, x, 64, None, None, 64, 0, many, x, v, None, None, None, None) == -1
+    for width, out, stride in ((0, 8, 8), (4097, 8, 8), (64, 0, 8), (64, 4097, 5000), (64, 8, 7)):
+        assert wgrad(x, x, None, None, None, None, width, 0, x, stride, out, acs, v, None, None) == -2
+    assert wgrad(x, x, None, None, None, None, 64, 0, x, 8, 8, acs, None, None, None) == wgrad(x, x, None, None, v, None, 64, 0, x, 8, 8, acs, v, None, None) == -1
+    assert wgrad(x, x + 4, None, None, None, None, 64, 0, x, 8, 8, acs, v, None, None) == -9
+    assert wgrad(x, x, None, None, None, None, 64, 0, x, 8, 8, many, v, None, None) == -1
+
+
+def test_there_is_no_cpu_path():
+    x, g = torch.zeros(3, 4), torch.ones(4)
+    for call in (lambda: layer_mod.layer_norm(x, g, g), lambda: layer_mod.layer_norm_grad(x, x, g, x[:, 0], x[:, 0]),
+                 lambda: layer_mod.checkpoint_activation(x, "celu")):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+    kept = layer_mod.ActivationCheckpoint(torch.zeros((3, 16), dtype=torch.uint8), torch.zeros((3, 1, 2)), 4, "celu")
+    for call in (layer_mod.checkpoint_activation_grad, layer_mod.checkpoint_weight_grad):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call(kept, x)
+    with pytest.raises(ValueError, match="activation"):
+        layer_mod.ActivationCheckpoint(kept.codes, kept.blocks, 4, "relu")
+
+
+def test_reference_norm_agrees_with_torch_in_double():
+    rng = np.random.default_rng(0)
+    x, up = rng.standard_normal((9, 13)), rng.standard_normal((9, 13))
+    gain, bias = [list(rng.standard_normal((4, 13))) for _ in range(2)]
+    acs = np.array([4, 0, 3, 2])
+    (y, mean, rstd), _ = ref.norm(x, gain, bias, acs, 1e-3)
+    (dx, dg, db), _ = ref.norm_grad(up, x, gain, mean.astype(float), rstd.astype(float), acs)
+    for t, rows in enumerate(ref.element_rows(acs)):
+        xt, g, b = (torch.from_numpy(np.asarray(v)).requires_grad_(True) for v in (x[rows], gain[t], bias[t]))
+        out = torch.nn.functional.layer_norm(xt, (13,), g, b, 1e-3)
+        out.backward(torch.from_numpy(up[rows]))
+        for got, want in ((y[rows], out.detach()), (dx[rows], xt.grad), (dg[t], g.grad), (db[t], b.grad)):
+            assert np.allclose(got.astype(float), want.numpy(), rtol=0, atol=1e-12)
+
+
+def test_reference_activations_agree_with_the_framework_in_double():
+    from khan_b200.model import activations
+    u = torch.linspace(-6, 6, 2001, dtype=torch.float64, requires_grad=True)
+    for name in activations.get_all_fn_names():
+        a = activations.get_fn_by_name(name)(u)
+        (d,) = torch.autograd.grad(a.sum(), u)
+        value, slope, second = ref.act(name, u.detach().numpy().astype(ref.LD))
+        assert np.abs(value - a.detach().numpy()).max() < 1e-14 and np.abs(slope - d.numpy()).max() < 1e-14
+        assert np.abs(np.diff(slope)).max() <= second * 0.006 * (1 + 1e-9)
+
+
+def test_reference_codes_stand_for_the_values():
+    rng = np.random.default_rng(1)
+    z = (rng.standard_normal((30, 300)) * 5 + 100).astype(np.float32)
+    codes, blocks = ref.encode(z)
+    step = blocks[:, np.arange(300) // 128, 1]
+    assert (np.abs(ref.decode(codes, blocks) - z) <= step * (0.5 + 1e-4)).all() and codes.max() == 255 and codes.min() == 0
