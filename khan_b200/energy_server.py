@@ -108,9 +108,12 @@ def main(argv=None) -> None:
     save_file = os.path.join(args.save_dir, "save_file.npz")
     if not os.path.exists(save_file):
         raise IOError("Saved NN numpy file does not exist")
+    with np.load(save_file, allow_pickle=False) as saved:
+        normed = any("_gain_" in name for name in saved.files)      # networks with layer norms
     trainer = TrainerMultiTower(None, [torch.device("cuda", torch.cuda.current_device())],
                                 precision=args.precision, layer_sizes=(128, 128, 64, 1),
-                                activation_fn=activations.get_fn_by_name(args.activation_function))
+                                activation_fn=activations.get_fn_by_name(args.activation_function),
+                                layer_norm=normed)
     trainer.load_numpy(save_file, strict=False)
     if args.debug:
         print(f"Server listening on port {args.port}")

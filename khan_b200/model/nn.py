@@ -10,6 +10,11 @@ one to one.
 For float32 and the architecture 384-128-128-64-1 the forward pass of all four networks is one
 fused tensor-core kernel (``ani_mlp_forward_f32``); its backward pass and every other
 architecture or precision use torch's dense GEMMs on the GPU.
+
+Two options go beyond the reference, for networks that are deeper or wider than its own.  ``layer_norm``:
+every hidden layer is ``A = act(norm(A W + b))`` with a gain and a shift per column.
+``activation_checkpoints``: training keeps the input of every activation in 8 bits between the forward and
+the backward pass, instead of that input and the activation in 32 (:mod:`khan_b200.layer_mod`).
 """
 from __future__ import annotations
 
@@ -18,7 +23,7 @@ import ctypes
 import numpy as np
 import torch
 
-from .. import _lib
+from .. import _lib, layer_mod
 from . import activations
 
 FUSED_LAYERS = (384, 128, 128, 64, 1)
@@ -30,14 +35,16 @@ class AtomNN:
 
     def __init__(self, layer_sizes, precision=torch.float32, activation_fn=activations.celu,
                  atom_type: str = "", prefix: str = "", device="cuda", generator=None,
-                 init: str = "reference"):
+                 init: str = "reference", layer_norm: bool = False, norm_eps: float = 1e-5):
         assert precision in (torch.float32, torch.float64)
         assert layer_sizes[-1] == 1
         self.layer_sizes = tuple(int(v) for v in layer_sizes)
         self.precision = precision
         self.activation_fn = activation_fn
         self.atom_type = atom_type
+        self.layer_norm, self.norm_eps = bool(layer_norm), float(norm_eps)
         self.Ws, self.bs, self.names = [], [], []
+        self.gains, self.shifts, self.norm_names = [], [], []      # of the hidden layers' norms
         for idx in range(1, len(layer_sizes)):
             x, y = layer_sizes[idx - 1], layer_sizes[idx]
             # reference: N(0, sqrt(2 / (x + y))), khan/model/nn.py:45-59; "he": N(0, sqrt(2 / x))
@@ -47,15 +54,21 @@ class AtomNN:
             self.Ws.append(w.to(precision).to(device).requires_grad_(True))
             self.bs.append(torch.zeros(y, dtype=precision, device=device, requires_grad=True))
             self.names.append((prefix + "W" + name, prefix + "b" + name))
+            if self.layer_norm and idx < len(layer_sizes) - 1:
+                name = "_" + atom_type + "_" + str(y) + "_l" + str(idx)
+                self.gains.append(torch.ones(y, dtype=precision, device=device, requires_grad=True))
+                self.shifts.append(torch.zeros(y, dtype=precision, device=device, requires_grad=True))
+                self.norm_names.append((prefix + "gain" + name, prefix + "shift" + name))
 
     def get_parameters(self):
-        return self.Ws + self.bs
+        return self.Ws + self.bs + self.gains + self.shifts
 
     def named_parameters(self):
         out = {}
-        for (wn, bn), w, b in zip(self.names, self.Ws, self.bs):
-            out[wn + ":0"] = w
-            out[bn + ":0"] = b
+        for names, first, second in ((self.names, self.Ws, self.bs), (self.norm_names, self.gains, self.shifts)):
+            for (fn, sn), f, s in zip(names, first, second):
+                out[fn + ":0"] = f
+                out[sn + ":0"] = s
         return out
 
     def atom_energies(self, features: torch.Tensor) -> torch.Tensor:
@@ -65,6 +78,9 @@ class AtomNN:
         for k, (w, b) in enumerate(zip(self.Ws, self.bs)):
             a = a @ w + b
             if k != last:
+                if self.layer_norm:
+                    norm = layer_mod.layer_norm_autograd if a.is_cuda else layer_mod.dense_layer_norm
+                    a = norm(a, self.gains[k], self.shifts[k], eps=self.norm_eps)
                 a = self.activation_fn(a)
         return a.reshape(-1)
 
@@ -220,6 +236,73 @@ class _FusedMlp(torch.autograd.Function):
         return (grad_feat, None, None, None, None, *grads)
 
 
+class _CheckpointedStacks(torch.autograd.Function):
+    """The four atomic networks with 8-bit activation checkpoints: dense products by torch, activations, norms and the
+    weight gradients behind them by :mod:`khan_b200.layer_mod`.  Between the passes there are one byte and a little per
+    hidden activation, and the features.  Gradients are those of the weights; they see the checkpoints (half a step of
+    1/255 of a row's spread over 128 columns), the energies do not."""
+
+    @staticmethod
+    def forward(ctx, features, acs, act_id, eps, layers, normed, *params):
+        # params, layer by layer: four W, four b, and for a normalised hidden layer four gains, four shifts
+        ends = np.cumsum(acs).tolist()
+        ranges = list(zip([0] + ends[:-1], ends))
+        per_layer = _CheckpointedStacks._by_layer(params, layers, normed)
+        a, kept = features, []
+        for k, (ws, bs, gains, shifts) in enumerate(per_layer):
+            z = torch.empty((features.shape[0], ws[0].shape[1]), dtype=torch.float32, device=features.device)
+            for (s, e), w, b in zip(ranges, ws, bs):
+                if e > s:
+                    torch.addmm(b, a[s:e], w, out=z[s:e])
+            if k == layers - 1:
+                break
+            a, checkpoint = layer_mod.checkpoint_activation(z, act_id, gains, shifts, acs, eps)
+            kept.append(checkpoint)
+        ctx.save_for_backward(features, *params)
+        ctx.kept, ctx.ranges, ctx.acs, ctx.layers, ctx.normed = kept, ranges, acs, layers, normed
+        return z.reshape(-1)
+
+    @staticmethod
+    def _by_layer(params, layers, normed):
+        out, at = [], 0
+        for k in range(layers):
+            with_norm = normed and k < layers - 1
+            group = [list(params[at + 4 * i: at + 4 * i + 4]) for i in range(4 if with_norm else 2)]
+            out.append((*group, *(() if with_norm else (None, None))))
+            at += 4 * len(group)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_energy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("a pass with activation checkpoints can be differentiated once: its activations are kept in "
+                               "8 bits (build the network without activation_checkpoints for higher derivatives)")
+        features, *params = ctx.saved_tensors
+        acs, ranges, layers = ctx.acs, ctx.ranges, ctx.layers
+        per_layer = _CheckpointedStacks._by_layer(params, layers, ctx.normed)
+        grads = [None] * layers
+        dz = grad_energy.reshape(-1, 1)
+        dsum = torch.stack([dz[s:e].sum(0) for s, e in ranges])
+        norm_grads = ()
+        for k in range(layers - 1, -1, -1):
+            ws = per_layer[k][0]
+            if k == 0:
+                dws = [features[s:e].t() @ dz[s:e] for s, e in ranges]
+            else:
+                gains, shifts = per_layer[k - 1][2:]
+                dws = layer_mod.checkpoint_weight_grad(ctx.kept[k - 1], dz, gains, shifts, acs)
+            grads[k] = [*dws, *dsum, *(g for four in norm_grads for g in four)]
+            if k == 0:
+                break
+            da = torch.empty((features.shape[0], ws[0].shape[0]), dtype=torch.float32, device=features.device)
+            for (s, e), w in zip(ranges, ws):
+                if e > s:
+                    torch.mm(dz[s:e], w.t(), out=da[s:e])
+            dz, dsum, *norm_grads = layer_mod.checkpoint_activation_grad(ctx.kept[k - 1], da, gains, shifts, acs)
+            norm_grads = norm_grads if ctx.normed else ()
+        return (None,) * 6 + tuple(g for layer in grads for g in layer)
+
+
 class _GatherRows(torch.autograd.Function):
     """``x[idx]`` whose backward is one scatter-add (torch's own index backward sorts the
     indices first: five launches instead of two)."""
@@ -242,16 +325,26 @@ class MoleculeNN:
 
     def __init__(self, type_map=TYPE_MAP, layer_sizes=FUSED_LAYERS, precision=torch.float32,
                  activation_fn=activations.celu, prefix: str = "near_", device="cuda", seed=None,
-                 init: str = "reference", split_precision: bool = True):
+                 init: str = "reference", split_precision: bool = True, layer_norm: bool = False,
+                 norm_eps: float = 1e-5, activation_checkpoints: bool = False):
+        if activation_checkpoints and (precision != torch.float32 or activation_fn not in activations.KERNEL_ID
+                                       or len(type_map) != 4 or len(layer_sizes) < 3):
+            raise ValueError("activation checkpoints are for float32 networks of four elements with a hidden layer and one "
+                             f"of the activations {activations.get_all_fn_names()}")
+        if (layer_norm or activation_checkpoints) and max(layer_sizes[1:]) > layer_mod.MAX_WIDTH:
+            raise ValueError(f"layers of normalised or checkpointed networks have at most {layer_mod.MAX_WIDTH} columns")
         gen = torch.Generator().manual_seed(seed) if seed is not None else None
         self.type_map = list(type_map)
         self.layer_sizes = tuple(layer_sizes)
         self.precision = precision
         self.activation_fn = activation_fn
         self.split_precision = split_precision
+        self.layer_norm, self.norm_eps = bool(layer_norm), float(norm_eps)
+        self.activation_checkpoints = bool(activation_checkpoints)
         self.accumulate_into_grad = False   # see _FusedMlp.backward; set by trainers that call .backward()
         self.anns = [AtomNN(layer_sizes, precision, activation_fn, atom_type=t, prefix=prefix,
-                            device=device, generator=gen, init=init) for t in self.type_map]
+                            device=device, generator=gen, init=init, layer_norm=layer_norm, norm_eps=norm_eps)
+                     for t in self.type_map]
 
     def get_parameters(self):
         out = []
@@ -295,7 +388,7 @@ class MoleculeNN:
         """The architecture of the hand-written network kernels: in float32 all of them, in float64 the one
         that evaluates energies and their gradient (``ani_energy_pass_f64``)."""
         return (self.layer_sizes == FUSED_LAYERS and len(self.anns) == 4
-                and self.activation_fn in activations.KERNEL_ID)
+                and self.activation_fn in activations.KERNEL_ID and not self.layer_norm)
 
     @property
     def fused(self) -> bool:
@@ -305,6 +398,8 @@ class MoleculeNN:
         """Energies in element-sorted order from the ``[n_atoms, F]`` feature buffer laid out H
         rows, C rows, N rows, O rows."""
         acs = np.asarray(acs, dtype=np.int64)
+        if self.activation_checkpoints and features.is_cuda and torch.is_grad_enabled() and not features.requires_grad:
+            return self._checkpointed_energies(features, acs)
         if self.fused and features.is_cuda:
             params = []
             for a in self.anns:
@@ -316,9 +411,34 @@ class MoleculeNN:
             return _FusedMlp.apply(features, acs, activations.KERNEL_ID[self.activation_fn],
                                    flags, (self.activation_fn, packed), *params)
         starts = np.concatenate([[0], np.cumsum(acs)])
+        if self.layer_norm and len(self.anns) == 4 and features.is_cuda:
+            return self._normed_energies(features, acs, starts)
         parts = [ann.atom_energies(features[int(starts[t]):int(starts[t + 1])])
                  for t, ann in enumerate(self.anns)]
         return torch.cat(parts)
+
+    def _normed_energies(self, features, acs, starts):
+        """Dense products per element, every norm of the four elements as one operator."""
+        acs = acs.astype(np.int32)
+        a = features
+        for k in range(len(self.layer_sizes) - 1):
+            a = torch.cat([a[int(starts[t]):int(starts[t + 1])] @ ann.Ws[k] + ann.bs[k] for t, ann in enumerate(self.anns)])
+            if k < len(self.layer_sizes) - 2:
+                a = self.activation_fn(layer_mod.layer_norm_autograd(
+                    a, [ann.gains[k] for ann in self.anns], [ann.shifts[k] for ann in self.anns], acs, self.norm_eps))
+        return a.reshape(-1)
+
+    def _checkpointed_energies(self, features, acs):
+        """Training: the exact energies, and gradients of the weights from 8-bit checkpoints.  Gradients with respect to the
+        features (forces) are never formed this way: they would lose digits that a user sees."""
+        _lib.same_device(features.device, self.anns[0].Ws[0], where="MoleculeNN.atom_energies_sorted")
+        params = []
+        layers = len(self.layer_sizes) - 1
+        for k in range(layers):
+            lists = ["Ws", "bs"] + (["gains", "shifts"] if self.layer_norm and k < layers - 1 else [])
+            params.extend(getattr(ann, name)[k] for name in lists for ann in self.anns)
+        return _CheckpointedStacks.apply(features, acs.astype(np.int32), self.activation_fn, self.norm_eps, layers,
+                                         self.layer_norm, *params)
 
     def atom_outputs(self, features: torch.Tensor, acs, gather_idxs: torch.Tensor) -> torch.Tensor:
         """Atomic energies in atom order (``tf.gather(tf.concat(...), gather_idxs)``,

@@ -117,7 +117,7 @@ class TrainerMultiTower:
 
     def __init__(self, sess, towers, precision=torch.float32, layer_sizes=(128, 128, 64, 8, 1),
                  activation_fn=activations.celu, fit_charges=False, seed=None, init="reference",
-                 split_precision=True):
+                 split_precision=True, layer_norm=False, activation_checkpoints=False):
         assert fit_charges is False
         precision = {"float32": torch.float32, "float64": torch.float64}.get(str(precision), precision)
         assert precision in (torch.float32, torch.float64)
@@ -140,7 +140,8 @@ class TrainerMultiTower:
         # the parameters live on the (only) tower
         self.model = MoleculeNN(layer_sizes=(self.feat_size,) + tuple(layer_sizes), precision=precision,
                                 activation_fn=activation_fn, prefix="near_", device=self.towers[0],
-                                seed=seed, init=init, split_precision=split_precision)
+                                seed=seed, init=init, split_precision=split_precision, layer_norm=layer_norm,
+                                activation_checkpoints=activation_checkpoints)
         self.all_models = [self.model]
         self.parameters = self.model.get_parameters()
         self.learning_rate = 1e-3
@@ -254,6 +255,10 @@ class TrainerMultiTower:
         import warnings
         objs = np.load(npz_file, allow_pickle=False)
         named = self.model.named_parameters()
+        normed = any("_gain_" in k for k in objs.keys())
+        if normed != self.model.layer_norm and any(k in named for k in objs.keys()):
+            raise ValueError(f"load_numpy: {npz_file} holds networks {'with' if normed else 'without'} layer norms, this "
+                             f"trainer's are {'with' if self.model.layer_norm else 'without'}")
         if not isinstance(self.optimizer, FlatNadam):       # torch creates its slots at the first step
             for p in self.parameters:
                 if p not in self.optimizer.state:
@@ -353,7 +358,7 @@ class TrainerMultiTower:
         fused_names = {"train_op", "train_op_rmse", "train_op_mse", "unordered_l2s", "tower_l2s", "tower_exp_loss",
                        "tower_bids", "_device_l2s"}
         fused = (self.num_towers == 1 and isinstance(self.optimizer, FlatNadam) and self.model.fused
-                 and len(training) == 1 and training[0] != "train_op_forces" and set(names) <= fused_names
+                 and not self.model.activation_checkpoints and len(training) == 1 and training[0] != "train_op_forces" and set(names) <= fused_names
                  and packed.ys is not None and packed.num_mols() > 0)
         force_fit = (self.num_towers == 1 and isinstance(self.optimizer, FlatNadam) and self.model.fused
                      and training == ["train_op_forces"]

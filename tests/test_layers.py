@@ -124,3 +124,29 @@ def test_reference_codes_stand_for_the_values():
     codes, blocks = ref.encode(z)
     step = blocks[:, np.arange(300) // 128, 1]
     assert (np.abs(ref.decode(codes, blocks) - z) <= step * (0.5 + 1e-4)).all() and codes.max() == 255 and codes.min() == 0
+
+
+def test_networks_refuse_what_checkpoints_cannot_do():
+    from khan_b200.model.nn import MoleculeNN
+    for kw in (dict(precision=torch.float64), dict(activation_fn=torch.tanh), dict(type_map=["H", "C"]), dict(layer_sizes=(384, 1))):
+        with pytest.raises(ValueError, match="activation checkpoints"):
+            MoleculeNN(device="cpu", activation_checkpoints=True, **kw)
+    with pytest.raises(ValueError, match="4096"):
+        MoleculeNN(device="cpu", layer_norm=True, layer_sizes=(384, 4097, 1))
+
+
+def test_normed_networks_have_named_gains_and_shifts():
+    from khan_b200.model.nn import MoleculeNN
+    net = MoleculeNN(device="cpu", layer_norm=True, layer_sizes=(384, 32, 16, 1), seed=1)
+    names = net.named_parameters()
+    assert names["near_gain_H_32_l1:0"] is net.anns[0].gains[0] and names["near_shift_O_16_l2:0"] is net.anns[3].shifts[1]
+    assert sorted(map(id, names.values())) == sorted(map(id, net.get_parameters()))
+    plain = MoleculeNN(device="cpu", layer_sizes=(384, 32, 16, 1), seed=1)
+    assert sorted(plain.named_parameters()) == sorted(n for n in names if "gain" not in n and "shift" not in n)
+    x = torch.rand((5, 384))
+    u = x @ net.anns[0].Ws[0] + net.anns[0].bs[0]
+    a = torch.nn.functional.layer_norm(u, (32,), net.anns[0].gains[0], net.anns[0].shifts[0], 1e-5)
+    a = net.activation_fn(a) @ net.anns[0].Ws[1] + net.anns[0].bs[1]
+    a = torch.nn.functional.layer_norm(a, (16,), net.anns[0].gains[1], net.anns[0].shifts[1], 1e-5)
+    want = (net.activation_fn(a) @ net.anns[0].Ws[2] + net.anns[0].bs[2]).reshape(-1)
+    assert torch.allclose(net.atom_energies_sorted(x, [5, 0, 0, 0]), want, atol=1e-5)
