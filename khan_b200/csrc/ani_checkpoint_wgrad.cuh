@@ -1,12 +1,22 @@
-// Weight gradient of the dense layer behind a checkpointed activation (ani_checkpoint.cuh):
+// Weight gradient of the dense layer behind a checkpointed activation (ani_checkpoint.cuh), on the tensor cores:
 //   dW = sum over the rows of an element  act(u~)^T dz   [width, out],  u~ from the codes as in the backward pass.
 // The activations are never in memory: a row's bytes become activations on their way into the product.
 //
-// K, the long axis, is the atom; a CTA takes a range of rows of one element and one tile of the output, and where an
-// element has several ranges they write partial products that a second launch adds in order.
+// K, the long axis, is the atom.  A CTA takes a range of rows of one element and a tile of 128 x 128 of the output, and
+// where an element has several ranges they write partial products that a second launch adds in order (no atomics).
+// Chunks of 32 rows are staged by four groups of 128 threads in turn.  A row's bytes and its part of dz come to shared
+// memory as bulk copies (rows of dz that are not 16-byte aligned by plain loads); then a thread has one column of A (a byte
+// per row: with the row's base, step, mean and rstd, two numbers a row, and its column's gain and bias the activation is two
+// FMAs and the function) and one column of B.  A goes to tensor memory, B to shared memory, both as tf32 high and low
+// parts; hi hi, hi lo and lo hi are three instructions per eight rows.
+//
+// The tensor core cuts a sum off at the accumulator's last place, always towards zero, so a long chain of additions drifts:
+// 1e-6 of the value per 32 additions.  So hi hi goes to two accumulators in turn, 128 rows to each, and while one is filled
+// the other is added to float32 sums; the small products (2^-11 of the large ones) have one accumulator for the whole range.
 #pragma once
 
 #include "ani_checkpoint.cuh"
+#include "ani_mlp_wgrad.cuh"
 
 namespace ani {
 
@@ -21,77 +31,261 @@ struct CheckpointWgradParams {
     float* grad_w[kTypes];      // [width][out]
     float* partial;             // [ranges][width][out]
     RowRanges ranges;
-    int width, out, act, norm;
+    int width, out, norm;
+    int bulk;                   // rows of grad_z are whole 16-byte pieces
 };
 
-constexpr int kCwTile = 64, kCwK = 16;
+constexpr int kCwTile = 128, kCwK = kPipeK;       // output tile, rows of a chunk
+static_assert(kCwTile == kCheckpointBlock, "the columns of a tile share their rows' base and step");
+constexpr int kCwRound = kChainGroups;            // chunks per accumulator: one of every group
+constexpr unsigned kCwMain = 0, kCwSmall = 256, kCwA = 384;      // tensor memory columns: two of 128, 128, two stages of 64
 
-__global__ void __launch_bounds__(256) checkpoint_wgrad_kernel(const __grid_constant__ CheckpointWgradParams p)
+struct CwShared {
+    alignas(1024) unsigned char b[kChainGroups][2 * kPipeOperandBytes];
+    alignas(16) unsigned char codes[kChainGroups][kCwK][kCwTile];      // a chunk's rows as they are
+    alignas(16) float dz[kChainGroups][kCwK][kCwTile];
+    alignas(16) float2 row[kMlpThreads / kWarp][kCwK];      // per warp: step rstd and (base - mean) rstd of the chunk's rows
+    alignas(8) unsigned long long rows[kChainGroups], full[kChainGroups], empty[kChainGroups], done[2], drained[2], end;
+    unsigned tmem_base;
+    int failed;
+};
+
+template <int ACT>
+__global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(const __grid_constant__ CheckpointWgradParams p)
 {
-    __shared__ alignas(16) float a[kCwK][kCwTile], b[kCwK][kCwTile];
+    extern __shared__ __align__(1024) unsigned char cw_smem_raw[];
+    CwShared& sh = *reinterpret_cast<CwShared*>(cw_smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const RowRange range = range_of_cta(p.ranges, blockIdx.x);
+    const int n_here = (int)(range.end - range.first);
+    const int m0 = blockIdx.y * kCwTile, n0 = blockIdx.z * kCwTile;
+    const int nchunks = (n_here + kCwK - 1) / kCwK, rounds = (nchunks + kCwRound - 1) / kCwRound;
+    const int n_columns = min(kCwTile, (p.out - n0 + 15) & ~15);      // of the instruction
+
+    if (warp == kMlpThreads / 32) tmem_alloc(&sh.tmem_base, 512);
+    if (tid == 0) {
+        for (int g = 0; g < kChainGroups; g++) {
+            mbar_init(&sh.rows[g], 1);
+            mbar_init(&sh.full[g], kMlpThreads / kChainGroups);
+            mbar_init(&sh.empty[g], 1);
+        }
+        for (int k = 0; k < 2; k++) {
+            mbar_init(&sh.done[k], 1);
+            mbar_init(&sh.drained[k], kMlpThreads);
+        }
+        mbar_init(&sh.end, 1);
+        sh.failed = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     pdl_wait();
     pdl_trigger();
-    const RowRange range = range_of_cta(p.ranges, blockIdx.x);
-    const int row_bytes = checkpoint_row_bytes(p.width), row_blocks = checkpoint_blocks(p.width);
-    const int m0 = blockIdx.y * kCwTile, n0 = blockIdx.z * kCwTile;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int col = threadIdx.x % kCwTile, k_in = threadIdx.x / kCwTile;
-    const int m = m0 + col, n = n0 + col;
-    const float gain = p.norm && m < p.width ? p.gain[range.element][m] : 1.0f;
-    const float bias = p.norm && m < p.width ? p.bias[range.element][m] : 0.0f;
-    float acc[4][4] = {};
-    for (long long r0 = range.first; r0 < range.end; r0 += kCwK) {
+    const unsigned tmem = sh.tmem_base;
+
+    if (warp == kMlpThreads / 32) {
+        // ---- the products: one thread ----
+        if (lane == 0) {
+            bool ok = true;
+            const unsigned idesc = instr_desc(kCwTile, n_columns);
+            for (int c = 0; c < nchunks && ok; c++) {
+                const int g = c % kChainGroups, r = c / kCwRound;
+                if (c % kCwRound == 0 && r >= 2) ok = mbar_wait(&sh.drained[r & 1], (unsigned)(r / 2 - 1) & 1u);
+                ok = ok && mbar_wait(&sh.full[g], (unsigned)(c / kChainGroups) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                const unsigned b_hi = smem_u32(sh.b[g]), b_lo = b_hi + kPipeOperandBytes;
+                const unsigned a_hi = tmem + kCwA + (c & 1) * 2 * kPipeK, a_lo = a_hi + kPipeK;
+                const unsigned acc = tmem + kCwMain + (r & 1) * 128;
 #pragma unroll
-        for (int k = k_in; k < kCwK; k += 4) {
-            const long long row = r0 + k;
-            float va = 0.0f, vb = 0.0f;
-            if (row < range.end) {
-                if (m < p.width) {
-                    const float2 block = p.blocks[row * row_blocks + m / kCheckpointBlock];
-                    float u = fmaf((float)p.codes[row * row_bytes + m], block.y, block.x);
-                    if (p.norm) u = (u - p.mean[row]) * p.rstd[row] * gain + bias;
-                    va = act_value(p.act, u);
+                for (int ks = 0; ks < kPipeK / 8; ks++) {
+                    const unsigned step = ks * 2 * kMlpLbo, col = ks * 8;
+                    mma_tf32_ts(acc, a_hi + col, pipe_desc(b_hi + step), idesc, !(c % kCwRound == 0 && ks == 0));
+                    mma_tf32_ts(tmem + kCwSmall, a_hi + col, pipe_desc(b_lo + step), idesc, !(c == 0 && ks == 0));
+                    mma_tf32_ts(tmem + kCwSmall, a_lo + col, pipe_desc(b_hi + step), idesc, true);
                 }
-                if (n < p.out) vb = p.grad_z[row * p.grad_stride + n];
+                mma_commit(&sh.empty[g]);
+                if (c % kCwRound == kCwRound - 1 || c == nchunks - 1) mma_commit(&sh.done[r & 1]);
             }
-            a[k][col] = va;
-            b[k][col] = vb;
+            if (ok) mma_commit(&sh.end);
+            else sh.failed = 1;
         }
-        __syncthreads();
+    } else {
+        // ---- staging: group g of 128 threads takes chunks g, g + 4, ...; every warp has 32 x 32 of the sums ----
+        const int g = warp >> 2, me = tid & 127;
+        const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
+        const int row_bytes = checkpoint_row_bytes(p.width), row_blocks = checkpoint_blocks(p.width);
+        const bool a_in = m0 + me < p.width, b_in = n0 + me < p.out;
+        const unsigned char* a_src = p.codes + range.first * row_bytes + m0;
+        const float* b_src = p.grad_z + range.first * p.grad_stride + n0;
+        const unsigned a_bytes = min(kCwTile, row_bytes - m0), b_bytes = p.bulk ? 4 * min(kCwTile, p.out - n0) : 0;
+        const float2* blocks = p.blocks + range.first * row_blocks + blockIdx.y;
+        // the copies of a chunk: a lane of the group's first warp has a row
+        auto fetch = [&](int c) {
+            const int k0 = c * kCwK, valid = min(kCwK, n_here - k0);
+            if (lane == 0) {
+                mbar_expect_tx(&sh.rows[g], valid * (a_bytes + b_bytes));
+                mbar_arrive(&sh.rows[g]);
+            }
+            __syncwarp();
+            if (lane < valid) {
+                bulk_copy_to_shared(sh.codes[g][lane], a_src + (size_t)(k0 + lane) * row_bytes, a_bytes, &sh.rows[g]);
+                if (b_bytes) bulk_copy_to_shared(sh.dz[g][lane], b_src + (size_t)(k0 + lane) * p.grad_stride, b_bytes, &sh.rows[g]);
+            }
+        };
+        if ((warp & 3) == 0 && g < nchunks) fetch(g);
+        const float gain = p.norm && a_in ? p.gain[range.element][m0 + me] : 1.0f;
+        const float bias = p.norm && a_in ? p.bias[range.element][m0 + me] : 0.0f;
+        bool timed_out = false;
+        float sum[32];
 #pragma unroll
-        for (int k = 0; k < kCwK; k++) {
-            const float4 x = *reinterpret_cast<const float4*>(&a[k][4 * ty]), y = *reinterpret_cast<const float4*>(&b[k][4 * tx]);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int i = 0; i < 32; i++) sum[i] = 0.0f;
+        auto drain = [&](int r) {
+            if (!timed_out) {
+                timed_out = !mbar_wait(&sh.done[r & 1], (unsigned)(r / 2) & 1u);
+                if (timed_out) sh.failed = 1;
+            }
+            __syncwarp();
+            tc_fence_after();
+            float v[32];
+            tmem_load32(lanes + kCwMain + (r & 1) * 128 + g * 32, v);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 32; i++) sum[i] += v[i];
+            tc_fence_before();
+            mbar_arrive(&sh.drained[r & 1]);
+        };
+        for (int r = 0; r < rounds; r++) {
+            const int c = r * kCwRound + g;
+            if (c < nchunks) {
+                const int k0 = c * kCwK, valid = min(kCwK, n_here - k0);
+                float2 scale = make_float2(0.0f, 0.0f);
+                if (lane < valid) {
+                    const float2 block = blocks[(size_t)(k0 + lane) * row_blocks];
+                    scale = make_float2(block.y, block.x);
+                    if (p.norm) {
+                        const float mean = p.mean[range.first + k0 + lane], rstd = p.rstd[range.first + k0 + lane];
+                        scale = make_float2(block.y * rstd, (block.x - mean) * rstd);
+                    }
+                }
+                __syncwarp();
+                sh.row[warp][lane] = scale;
+                __syncwarp();
+                if (!p.bulk) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xs[i], ys[j], acc[i][j]);
+                    for (int k0 = 0; k0 < kCwK; k0 += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++)
+                            v[k] = k0 + k < valid && b_in ? b_src[(size_t)(c * kCwK + k0 + k) * p.grad_stride + me] : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 16; k++) sh.dz[g][k0 + k][me] = v[k];      // read by this thread alone
+                    }
+                }
+                if (!mbar_wait(&sh.rows[g], (unsigned)r & 1u)) timed_out = true;
+                // chunk c - 2 had the stage of tensor memory, chunk c - 4, before it, that of shared memory
+                if (c >= 2 && !timed_out)
+                    timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
+                if (timed_out) sh.failed = 1;
+                __syncwarp();
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kCwK; k += 4) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = k + i < valid && b_in ? sh.dz[g][k + i][me] : 0.0f;
+                    pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k), make_float4(v[0], v[1], v[2], v[3]));
+                }
+                fence_async_smem();
+                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
+                // Columns behind the width: rows of the product that are not stored.
+                const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
+#pragma unroll
+                for (int k0 = 0; k0 < kCwK; k0 += 8) {
+                    float a[8], part[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const float4 s = *reinterpret_cast<const float4*>(&sh.row[warp][k0 + k]);
+                        a[k] = mlp_activation<ACT>(fmaf(fmaf((float)sh.codes[g][k0 + k][me], s.x, s.y), gain, bias));
+                        a[k + 1] = mlp_activation<ACT>(fmaf(fmaf((float)sh.codes[g][k0 + k + 1][me], s.z, s.w), gain, bias));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k]);
+                    tmem_store8(stage + k0, part);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) part[k] = a[k] - part[k];
+                    tmem_store8(stage + kPipeK + k0, part);
+                }
+                tmem_store_wait();
+                tc_fence_before();
+                mbar_arrive(&sh.full[g]);
+                if (c + kChainGroups < nchunks) {
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");      // the group has read the chunk's rows
+                    if ((warp & 3) == 0) fetch(c + kChainGroups);
+                }
+            }
+            if (r > 0) drain(r - 1);
         }
-        __syncthreads();
+        drain(rounds - 1);
+        bool ok = !timed_out;
+        if (ok && !mbar_wait(&sh.end, 0u)) {
+            ok = false;
+            sh.failed = 1;
+        }
+        __syncwarp();
+        tc_fence_after();
+        float small[32];
+        tmem_load32(lanes + kCwSmall + g * 32, small);
+        producer_sync();      // the operand stages become transposition scratch
+        if (ok && !sh.failed) {
+            const bool single = p.ranges.range_start[range.element + 1] - p.ranges.range_start[range.element] == 1;
+            float* out = single ? p.grad_w[range.element] : p.partial + (size_t)blockIdx.x * p.width * p.out;
+            float* scratch = reinterpret_cast<float*>(sh.b[0]) + warp * (32 * kMlpScratchStride);
+#pragma unroll
+            for (int i = 0; i < 32; i++) scratch[lane * kMlpScratchStride + i] = sum[i] + small[i];
+            __syncwarp();
+            const int column = n0 + g * 32 + lane, first = m0 + (warp & 3) * 32;
+            if (column < p.out)
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (first + i < p.width) out[(size_t)(first + i) * p.out + column] = scratch[i * kMlpScratchStride + lane];
+        }
     }
-    const bool single = p.ranges.range_start[range.element + 1] - p.ranges.range_start[range.element] == 1;
-    float* out = single ? p.grad_w[range.element] : p.partial + (size_t)blockIdx.x * p.width * p.out;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int row = m0 + 4 * ty + i, c = n0 + 4 * tx + j;
-            if (row < p.width && c < p.out) out[(size_t)row * p.out + c] = acc[i][j];
-        }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && sh.failed) report(ANI_ERR_TIMEOUT);
+    tc_fence_after();
+    if (warp == kMlpThreads / 32) tmem_dealloc(tmem, 512);
 }
 
-// The partial products of an element's ranges, added in order; zeros for an element without rows.
-__global__ void __launch_bounds__(256) checkpoint_wgrad_sum_kernel(const __grid_constant__ CheckpointWgradParams p)
+// The partial products of an element's ranges, added in order: eight threads have a part of the ranges each, four values at
+// a time, and their sums are added in order too.  Zeros for an element without rows.
+constexpr int kCwSumLanes = 32, kCwSumParts = 8;
+__global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum_kernel(const __grid_constant__ CheckpointWgradParams p)
 {
+    __shared__ alignas(16) float part[kCwSumParts][4 * kCwSumLanes];
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.y, first = p.ranges.range_start[t], n = p.ranges.range_start[t + 1] - first;
     if (n == 1 || !p.grad_w[t]) return;      // written already, or an element without rows and without a place
-    const size_t size = (size_t)p.width * p.out;
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < size; i += (size_t)gridDim.x * blockDim.x) {
-        float s = 0.0f;
-        for (int k = 0; k < n; k++) s += p.partial[(size_t)(first + k) * size + i];
-        p.grad_w[t][i] = s;
+    const int size = p.width * p.out, at = 4 * (blockIdx.x * kCwSumLanes + threadIdx.x);
+    const bool vec = size % 4 == 0;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int each = (n + kCwSumParts - 1) / kCwSumParts, begin = threadIdx.y * each, end = min(n, begin + each);
+#pragma unroll 4
+    for (int k = begin; k < end; k++) {
+        float v[4];
+        load_columns(p.partial + (size_t)(first + k) * size, at, size, vec, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] += v[i];
+    }
+    store4(&part[threadIdx.y][4 * threadIdx.x], s);
+    __syncthreads();
+    const int i = threadIdx.y * kCwSumLanes + threadIdx.x, value = blockIdx.x * 4 * kCwSumLanes + i;
+    if (i < 4 * kCwSumLanes && value < size) {
+        float total = part[0][i];
+#pragma unroll
+        for (int k = 1; k < kCwSumParts; k++) total += part[k][i];
+        p.grad_w[t][value] = total;
     }
 }
 

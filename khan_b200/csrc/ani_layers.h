@@ -70,7 +70,7 @@ int rows_at_once(int width)
 // Ranges of the launches with sums over rows.
 RowRanges sum_ranges(const int* acs, int width)
 {
-    return row_ranges(acs, 2 * kNormSms, rows_at_once(width), 4 * rows_at_once(width));
+    return row_ranges(acs, 2 * kSms, rows_at_once(width), 4 * rows_at_once(width));
 }
 size_t sums_workspace(const RowRanges& r, int sums, int width, size_t size)
 {
@@ -159,13 +159,38 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
 
 bool known_activation(int act) { return act >= kActCelu && act <= kActSoftplus; }
 
-// Output tiles and ranges of the weight gradient.
+// Ranges of the weight gradient: a CTA holds an SM, so the ranges of all tiles are to fill whole waves of SMs.  Of one to
+// four waves the one with the least work in a CTA is taken; setting up a CTA and writing its tile costs about as much as 128
+// rows.
 RowRanges wgrad_ranges(const int* acs, int width, int out)
 {
     const long long tiles = (long long)((width + kCwTile - 1) / kCwTile) * ((out + kCwTile - 1) / kCwTile);
-    return row_ranges(acs, std::max<long long>(1, 4 * kNormSms / tiles), kCwK, 4 * kCwK);
+    int elements = 0;
+    long long most = 0;
+    for (int t = 0; t < kTypes; t++) {
+        elements += acs[t] > 0;
+        most = std::max<long long>(most, acs[t]);
+    }
+    long long best = -1, best_rows = (most + kCwK - 1) / kCwK * kCwK;
+    for (int waves = 1; waves <= 4; waves++) {
+        const long long budget = (long long)waves * kSms / tiles;      // ranges
+        if (budget < elements) continue;
+        long long low = 1, high = std::max<long long>(1, (most + kCwK - 1) / kCwK);      // chunks per range
+        while (low < high) {
+            const long long mid = (low + high) / 2;
+            long long count = 0;
+            for (int t = 0; t < kTypes; t++) count += (acs[t] + mid * kCwK - 1) / (mid * kCwK);
+            if (count <= budget) high = mid;
+            else low = mid + 1;
+        }
+        const long long work = waves * (low * kCwK + 128);
+        if (best < 0 || work < best) {
+            best = work;
+            best_rows = low * kCwK;
+        }
+    }
+    return row_ranges(acs, 0x7fffffff, kCwK, std::max<long long>(kCwK, best_rows));
 }
-
 }  // namespace
 
 extern "C" {
@@ -293,17 +318,22 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     if (!one_range_each(p.ranges) && !workspace) return ANI_ERR_NULL_POINTER;
     p.codes = codes; p.blocks = reinterpret_cast<const float2*>(blocks); p.mean = mean; p.rstd = rstd;
     p.grad_z = grad_z; p.grad_stride = grad_stride; p.partial = static_cast<float*>(workspace);
-    p.width = width; p.out = out_width; p.act = activation; p.norm = gain_host != nullptr;
+    p.width = width; p.out = out_width; p.norm = gain_host != nullptr;
+    p.bulk = aligned16({grad_z}) && grad_stride % 4 == 0 && out_width % 4 == 0;
     if (n > 0) {
         const dim3 grid(p.ranges.range_start[kTypes], (width + kCwTile - 1) / kCwTile, (out_width + kCwTile - 1) / kCwTile);
-        ANI_CUDA(launch_chain(checkpoint_wgrad_kernel, grid, 256, 0, (cudaStream_t)stream, 1, p));
+        auto kernel = activation == kActCelu       ? checkpoint_wgrad_kernel<kActCelu>
+                      : activation == kActGaussian ? checkpoint_wgrad_kernel<kActGaussian>
+                      : activation == kActNormal   ? checkpoint_wgrad_kernel<kActNormal>
+                                                   : checkpoint_wgrad_kernel<kActSoftplus>;
+        if (int rc = set_smem(kernel, sizeof(CwShared))) return rc;
+        ANI_CUDA(launch_chain(kernel, grid, kMlpAllThreads, sizeof(CwShared), (cudaStream_t)stream, 1, p));
     }
     bool all_written = true;      // by that launch
     for (int t = 0; t < kTypes; t++) all_written = all_written && (acs_host[t] == 0 ? !p.grad_w[t] : p.ranges.range_start[t + 1] - p.ranges.range_start[t] == 1);
     if (all_written) return ANI_OK;
-    const size_t size = (size_t)width * out_width;
-    const dim3 sum_grid((unsigned)std::min<size_t>((size + 255) / 256, 4 * kNormSms), kTypes);
-    ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, 256, 0, (cudaStream_t)stream, 1, p));
+    const dim3 sum_grid((width * out_width + 4 * kCwSumLanes - 1) / (4 * kCwSumLanes), kTypes);
+    ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, dim3(kCwSumLanes, kCwSumParts), 0, (cudaStream_t)stream, 1, p));
     return ANI_OK;
 }
 size_t ani_checkpoint_weight_grad_workspace_bytes(int width, int out_width, const int* acs_host)

@@ -23,7 +23,6 @@ namespace ani {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxWidth = 4096;
-constexpr int kNormSms = 148;      // of a B200; the plans below only have to be good, not exact
 
 struct RowGroups {
     long long start[kTypes + 1];   // rows of element t: start[t] .. start[t + 1]
