@@ -24,19 +24,47 @@ constexpr int kCheckpointBlock = 128;
 __host__ __device__ __forceinline__ int checkpoint_row_bytes(int width) { return (width + 15) & ~15; }
 __host__ __device__ __forceinline__ int checkpoint_blocks(int width) { return (width + kCheckpointBlock - 1) / kCheckpointBlock; }
 
+// The activation functions on the special function unit's exponential (2^-22 of its value; the argument's rounding adds
+// |x| 2^-24): a few 1e-7 of max(1, |a|), in a quarter of the instructions of expf and log1pf.
+// log(1 + e) for e in [0, 1] = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series: what is cut off is below 2e-8 of it.
+__device__ __forceinline__ float log1p_unit(float e)
+{
+    const float s = __fdividef(e, 2.0f + e), t = s * s;
+    float p = 1.0f / 13.0f;
+    p = fmaf(p, t, 1.0f / 11.0f);
+    p = fmaf(p, t, 1.0f / 9.0f);
+    p = fmaf(p, t, 1.0f / 7.0f);
+    p = fmaf(p, t, 0.2f);
+    p = fmaf(p, t, 1.0f / 3.0f);
+    return 2.0f * fmaf(p * t, s, s);
+}
+template <int ACT> __device__ __forceinline__ float act_value(float u)
+{
+    if (ACT == kActCelu) return u >= 0.0f ? u : fmaf(0.1f, __expf(10.0f * u), -0.1f);
+    if (ACT == kActGaussian) return __expf(-u * u);
+    if (ACT == kActNormal) return __expf(-0.5f * u * u);
+    return fmaxf(u, 0.0f) + log1p_unit(__expf(-fabsf(u))) - 0.69314718056f;
+}
+template <int ACT> __device__ __forceinline__ float act_derivative(float u)
+{
+    if (ACT == kActCelu) return u >= 0.0f ? 1.0f : __expf(10.0f * u);
+    if (ACT == kActGaussian) return -2.0f * u * __expf(-u * u);
+    if (ACT == kActNormal) return -u * __expf(-0.5f * u * u);
+    return __fdividef(1.0f, 1.0f + __expf(-u));
+}
 __device__ __forceinline__ float act_value(int act, float u)
 {
-    if (act == kActCelu) return mlp_activation<kActCelu>(u);
-    if (act == kActGaussian) return mlp_activation<kActGaussian>(u);
-    if (act == kActNormal) return mlp_activation<kActNormal>(u);
-    return mlp_activation<kActSoftplus>(u);
+    if (act == kActCelu) return act_value<kActCelu>(u);
+    if (act == kActGaussian) return act_value<kActGaussian>(u);
+    if (act == kActNormal) return act_value<kActNormal>(u);
+    return act_value<kActSoftplus>(u);
 }
 __device__ __forceinline__ float act_derivative(int act, float u)
 {
-    if (act == kActCelu) return u >= 0.0f ? 1.0f : expf(u * 10.0f);
-    if (act == kActGaussian) return -2.0f * u * expf(-u * u);
-    if (act == kActNormal) return -u * expf(-0.5f * u * u);
-    return 1.0f / (1.0f + expf(-u));
+    if (act == kActCelu) return act_derivative<kActCelu>(u);
+    if (act == kActGaussian) return act_derivative<kActGaussian>(u);
+    if (act == kActNormal) return act_derivative<kActNormal>(u);
+    return act_derivative<kActSoftplus>(u);
 }
 
 // Smaller / larger of two values, NaN if one of them is.

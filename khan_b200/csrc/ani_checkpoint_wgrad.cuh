@@ -15,6 +15,8 @@
 // the other is added to float32 sums; the small products (2^-11 of the large ones) have one accumulator for the whole range.
 #pragma once
 
+#include <type_traits>
+
 #include "ani_checkpoint.cuh"
 #include "ani_mlp_wgrad.cuh"
 
@@ -154,22 +156,34 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
             tc_fence_before();
             mbar_arrive(&sh.drained[r & 1]);
         };
+        // step rstd and (base - mean) rstd of the chunk's row `lane`, read a turn ahead
+        float2 block = make_float2(0.0f, 0.0f);
+        float mean = 0.0f, rstd = 1.0f;
+        auto read_row = [&](int c) {
+            const int k = c * kCwK + lane;
+            const bool live = k < n_here;
+            block = live ? blocks[(size_t)k * row_blocks] : make_float2(0.0f, 0.0f);
+            mean = live && p.norm ? p.mean[range.first + k] : 0.0f;
+            rstd = live && p.norm ? p.rstd[range.first + k] : 1.0f;
+        };
+        // the column of B of a chunk, `valid` of whose rows are in the range
+        auto store_b = [&](auto whole, int valid) {
+#pragma unroll
+            for (int k = 0; k < kCwK; k += 4) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = decltype(whole)::value || k + i < valid ? sh.dz[g][k + i][me] : 0.0f;
+                pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k), make_float4(v[0], v[1], v[2], v[3]));
+            }
+        };
+        read_row(g);
         for (int r = 0; r < rounds; r++) {
             const int c = r * kCwRound + g;
             if (c < nchunks) {
-                const int k0 = c * kCwK, valid = min(kCwK, n_here - k0);
-                float2 scale = make_float2(0.0f, 0.0f);
-                if (lane < valid) {
-                    const float2 block = blocks[(size_t)(k0 + lane) * row_blocks];
-                    scale = make_float2(block.y, block.x);
-                    if (p.norm) {
-                        const float mean = p.mean[range.first + k0 + lane], rstd = p.rstd[range.first + k0 + lane];
-                        scale = make_float2(block.y * rstd, (block.x - mean) * rstd);
-                    }
-                }
+                const int valid = min(kCwK, n_here - c * kCwK);
+                sh.row[warp][lane] = make_float2(block.y * rstd, (block.x - mean) * rstd);
                 __syncwarp();
-                sh.row[warp][lane] = scale;
-                __syncwarp();
+                if (c + kChainGroups < nchunks) read_row(c + kChainGroups);
                 if (!p.bulk) {
 #pragma unroll
                     for (int k0 = 0; k0 < kCwK; k0 += 16) {
@@ -182,37 +196,36 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                     }
                 }
                 if (!mbar_wait(&sh.rows[g], (unsigned)r & 1u)) timed_out = true;
-                // chunk c - 2 had the stage of tensor memory, chunk c - 4, before it, that of shared memory
+                // the products of the group's chunk before read this stage of shared memory
+                if (r > 0 && !timed_out) timed_out = !mbar_wait(&sh.empty[g], (unsigned)(r - 1) & 1u);
+                // columns behind the width of dz: columns of the product that are not stored
+                if (valid == kCwK) store_b(std::true_type(), valid);
+                else store_b(std::false_type(), valid);
+                fence_async_smem();
+                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
+                // Columns behind the width: rows of the product that are not stored.
+                float a[kCwK];
+#pragma unroll
+                for (int k = 0; k < kCwK; k += 2) {
+                    const float4 s = *reinterpret_cast<const float4*>(&sh.row[warp][k]);
+                    a[k] = act_value<ACT>(fmaf(fmaf((float)sh.codes[g][k][me], s.x, s.y), gain, bias));
+                    a[k + 1] = act_value<ACT>(fmaf(fmaf((float)sh.codes[g][k + 1][me], s.z, s.w), gain, bias));
+                }
+                // and those of chunk c - 2 this stage of tensor memory
                 if (c >= 2 && !timed_out)
                     timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
                 if (timed_out) sh.failed = 1;
                 __syncwarp();
                 tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < kCwK; k += 4) {
-                    float v[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = k + i < valid && b_in ? sh.dz[g][k + i][me] : 0.0f;
-                    pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k), make_float4(v[0], v[1], v[2], v[3]));
-                }
-                fence_async_smem();
-                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
-                // Columns behind the width: rows of the product that are not stored.
                 const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
 #pragma unroll
                 for (int k0 = 0; k0 < kCwK; k0 += 8) {
-                    float a[8], part[8];
+                    float part[8];
 #pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        const float4 s = *reinterpret_cast<const float4*>(&sh.row[warp][k0 + k]);
-                        a[k] = mlp_activation<ACT>(fmaf(fmaf((float)sh.codes[g][k0 + k][me], s.x, s.y), gain, bias));
-                        a[k + 1] = mlp_activation<ACT>(fmaf(fmaf((float)sh.codes[g][k0 + k + 1][me], s.z, s.w), gain, bias));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k]);
+                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k0 + k]);
                     tmem_store8(stage + k0, part);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = a[k] - part[k];
+                    for (int k = 0; k < 8; k++) part[k] = a[k0 + k] - part[k];
                     tmem_store8(stage + kPipeK + k0, part);
                 }
                 tmem_store_wait();
