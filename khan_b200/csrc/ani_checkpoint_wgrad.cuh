@@ -4,18 +4,17 @@
 //
 // K, the long axis, is the atom.  A CTA takes a range of rows of one element and a tile of 128 x 128 of the output, and
 // where an element has several ranges they write partial products that a second launch adds in order (no atomics).
-// Chunks of 32 rows are staged by four groups of 128 threads in turn.  A row's bytes and its part of dz come to shared
-// memory as bulk copies (rows of dz that are not 16-byte aligned by plain loads); then a thread has one column of A (a byte
-// per row: with the row's base, step, mean and rstd, two numbers a row, and its column's gain and bias the activation is two
-// FMAs and the function) and one column of B.  A goes to tensor memory, B to shared memory, both as tf32 high and low
-// parts; hi hi, hi lo and lo hi are three instructions per eight rows.
+// Chunks of 32 rows are staged by four groups of 128 threads in turn.  A chunk's bytes and its part of dz come to shared
+// memory by asynchronous copies of 16 bytes (4 where rows of dz are not aligned), asked for when the group has read the
+// chunk before.  (Bulk copies of a row each, 64 a chunk, took the issuing warp 5000 clocks and everybody's shared-memory
+// reads with it.)  Then a thread has one column of A (a byte per row: with the row's base, step, mean and rstd, two numbers
+// a row, and its column's gain and bias the activation is two FMAs and the function) and one column of B.  A goes to tensor
+// memory, B to shared memory, both as tf32 high and low parts; hi hi, hi lo and lo hi are three instructions per eight rows.
 //
 // The tensor core cuts a sum off at the accumulator's last place, always towards zero, so a long chain of additions drifts:
 // 1e-6 of the value per 32 additions.  So hi hi goes to two accumulators in turn, 128 rows to each, and while one is filled
 // the other is added to float32 sums; the small products (2^-11 of the large ones) have one accumulator for the whole range.
 #pragma once
-
-#include <type_traits>
 
 #include "ani_checkpoint.cuh"
 #include "ani_mlp_wgrad.cuh"
@@ -34,7 +33,7 @@ struct CheckpointWgradParams {
     float* partial;             // [ranges][width][out]
     RowRanges ranges;
     int width, out, norm;
-    int bulk;                   // rows of grad_z are whole 16-byte pieces
+    int whole;                  // rows of grad_z are whole 16-byte pieces
 };
 
 constexpr int kCwTile = 128, kCwK = kPipeK;       // output tile, rows of a chunk
@@ -42,12 +41,22 @@ static_assert(kCwTile == kCheckpointBlock, "the columns of a tile share their ro
 constexpr int kCwRound = kChainGroups;            // chunks per accumulator: one of every group
 constexpr unsigned kCwMain = 0, kCwSmall = 256, kCwA = 384;      // tensor memory columns: two of 128, 128, two stages of 64
 
+// 16 or 4 bytes to shared memory; the last `size` .. BYTES of them are zeros, and with size 0 nothing is read.
+template <int BYTES> __device__ __forceinline__ void copy_async(void* dst_smem, const void* src, int size)
+{
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst_smem)), "l"(src), "r"(size) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst_smem)), "l"(src), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 struct CwShared {
     alignas(1024) unsigned char b[kChainGroups][2 * kPipeOperandBytes];
     alignas(16) unsigned char codes[kChainGroups][kCwK][kCwTile];      // a chunk's rows as they are
     alignas(16) float dz[kChainGroups][kCwK][kCwTile];
     alignas(16) float2 row[kMlpThreads / kWarp][kCwK];      // per warp: step rstd and (base - mean) rstd of the chunk's rows
-    alignas(8) unsigned long long rows[kChainGroups], full[kChainGroups], empty[kChainGroups], done[2], drained[2], end;
+    alignas(8) unsigned long long full[kChainGroups], empty[kChainGroups], done[2], drained[2], end;
     unsigned tmem_base;
     int failed;
 };
@@ -67,7 +76,6 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
     if (warp == kMlpThreads / 32) tmem_alloc(&sh.tmem_base, 512);
     if (tid == 0) {
         for (int g = 0; g < kChainGroups; g++) {
-            mbar_init(&sh.rows[g], 1);
             mbar_init(&sh.full[g], kMlpThreads / kChainGroups);
             mbar_init(&sh.empty[g], 1);
         }
@@ -117,25 +125,34 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
         const int g = warp >> 2, me = tid & 127;
         const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
         const int row_bytes = checkpoint_row_bytes(p.width), row_blocks = checkpoint_blocks(p.width);
-        const bool a_in = m0 + me < p.width, b_in = n0 + me < p.out;
+        const bool a_in = m0 + me < p.width;
         const unsigned char* a_src = p.codes + range.first * row_bytes + m0;
         const float* b_src = p.grad_z + range.first * p.grad_stride + n0;
-        const unsigned a_bytes = min(kCwTile, row_bytes - m0), b_bytes = p.bulk ? 4 * min(kCwTile, p.out - n0) : 0;
+        const int a_bytes = min(kCwTile, row_bytes - m0), b_columns = min(kCwTile, p.out - n0);
         const float2* blocks = p.blocks + range.first * row_blocks + blockIdx.y;
-        // the copies of a chunk: a lane of the group's first warp has a row
+        // the copies of a chunk, by the group; rows of dz behind the range are zeros, bytes there are left as they are
         auto fetch = [&](int c) {
             const int k0 = c * kCwK, valid = min(kCwK, n_here - k0);
-            if (lane == 0) {
-                mbar_expect_tx(&sh.rows[g], valid * (a_bytes + b_bytes));
-                mbar_arrive(&sh.rows[g]);
+#pragma unroll
+            for (int i = 0; i < kCwK * kCwTile / 16 / 128; i++) {
+                const int row = (i * 128 + me) / (kCwTile / 16), at = 16 * (me % (kCwTile / 16));
+                if (row < valid && at < a_bytes) copy_async<16>(&sh.codes[g][row][at], a_src + (size_t)(k0 + row) * row_bytes + at, 16);
             }
-            __syncwarp();
-            if (lane < valid) {
-                bulk_copy_to_shared(sh.codes[g][lane], a_src + (size_t)(k0 + lane) * row_bytes, a_bytes, &sh.rows[g]);
-                if (b_bytes) bulk_copy_to_shared(sh.dz[g][lane], b_src + (size_t)(k0 + lane) * p.grad_stride, b_bytes, &sh.rows[g]);
+            if (p.whole) {
+#pragma unroll
+                for (int i = 0; i < kCwK * kCwTile / 4 / 128; i++) {
+                    const int row = (i * 128 + me) / (kCwTile / 4), at = 4 * (me % (kCwTile / 4));
+                    if (at < b_columns)
+                        copy_async<16>(&sh.dz[g][row][at], b_src + (row < valid ? (size_t)(k0 + row) * p.grad_stride + at : 0), row < valid ? 16 : 0);
+                }
+            } else if (me < b_columns) {
+#pragma unroll 8
+                for (int row = 0; row < kCwK; row++)
+                    copy_async<4>(&sh.dz[g][row][me], b_src + (row < valid ? (size_t)(k0 + row) * p.grad_stride + me : 0), row < valid ? 4 : 0);
             }
         };
-        if ((warp & 3) == 0 && g < nchunks) fetch(g);
+        auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
+        if (g < nchunks) fetch(g);
         const float gain = p.norm && a_in ? p.gain[range.element][m0 + me] : 1.0f;
         const float bias = p.norm && a_in ? p.bias[range.element][m0 + me] : 0.0f;
         bool timed_out = false;
@@ -166,41 +183,21 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
             mean = live && p.norm ? p.mean[range.first + k] : 0.0f;
             rstd = live && p.norm ? p.rstd[range.first + k] : 1.0f;
         };
-        // the column of B of a chunk, `valid` of whose rows are in the range
-        auto store_b = [&](auto whole, int valid) {
-#pragma unroll
-            for (int k = 0; k < kCwK; k += 4) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = decltype(whole)::value || k + i < valid ? sh.dz[g][k + i][me] : 0.0f;
-                pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k), make_float4(v[0], v[1], v[2], v[3]));
-            }
-        };
         read_row(g);
         for (int r = 0; r < rounds; r++) {
             const int c = r * kCwRound + g;
             if (c < nchunks) {
-                const int valid = min(kCwK, n_here - c * kCwK);
                 sh.row[warp][lane] = make_float2(block.y * rstd, (block.x - mean) * rstd);
-                __syncwarp();
+                copies_wait();
+                group_sync();      // everybody's copies
                 if (c + kChainGroups < nchunks) read_row(c + kChainGroups);
-                if (!p.bulk) {
-#pragma unroll
-                    for (int k0 = 0; k0 < kCwK; k0 += 16) {
-                        float v[16];
-#pragma unroll
-                        for (int k = 0; k < 16; k++)
-                            v[k] = k0 + k < valid && b_in ? b_src[(size_t)(c * kCwK + k0 + k) * p.grad_stride + me] : 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 16; k++) sh.dz[g][k0 + k][me] = v[k];      // read by this thread alone
-                    }
-                }
-                if (!mbar_wait(&sh.rows[g], (unsigned)r & 1u)) timed_out = true;
                 // the products of the group's chunk before read this stage of shared memory
                 if (r > 0 && !timed_out) timed_out = !mbar_wait(&sh.empty[g], (unsigned)(r - 1) & 1u);
                 // columns behind the width of dz: columns of the product that are not stored
-                if (valid == kCwK) store_b(std::true_type(), valid);
-                else store_b(std::false_type(), valid);
+#pragma unroll
+                for (int k = 0; k < kCwK; k += 4)
+                    pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k),
+                                      make_float4(sh.dz[g][k][me], sh.dz[g][k + 1][me], sh.dz[g][k + 2][me], sh.dz[g][k + 3][me]));
                 fence_async_smem();
                 // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
                 // Columns behind the width: rows of the product that are not stored.
@@ -232,8 +229,8 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                 tc_fence_before();
                 mbar_arrive(&sh.full[g]);
                 if (c + kChainGroups < nchunks) {
-                    asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");      // the group has read the chunk's rows
-                    if ((warp & 3) == 0) fetch(c + kChainGroups);
+                    group_sync();      // the group has read the chunk's rows
+                    fetch(c + kChainGroups);
                 }
             }
             if (r > 0) drain(r - 1);

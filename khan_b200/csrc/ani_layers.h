@@ -319,7 +319,7 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     p.codes = codes; p.blocks = reinterpret_cast<const float2*>(blocks); p.mean = mean; p.rstd = rstd;
     p.grad_z = grad_z; p.grad_stride = grad_stride; p.partial = static_cast<float*>(workspace);
     p.width = width; p.out = out_width; p.norm = gain_host != nullptr;
-    p.bulk = aligned16({grad_z}) && grad_stride % 4 == 0 && out_width % 4 == 0;
+    p.whole = aligned16({grad_z}) && grad_stride % 4 == 0 && out_width % 4 == 0;
     if (n > 0) {
         const dim3 grid(p.ranges.range_start[kTypes], (width + kCwTile - 1) / kCwTile, (out_width + kCwTile - 1) / kCwTile);
         auto kernel = activation == kActCelu       ? checkpoint_wgrad_kernel<kActCelu>
