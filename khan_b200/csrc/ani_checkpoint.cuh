@@ -67,19 +67,52 @@ template <int ACT> __device__ __forceinline__ float act_derivative(float u)
     if (ACT == kActNormal) return -u * __expf(-0.5f * u * u);
     return __fdividef(1.0f, 1.0f + __expf(-u));
 }
-__device__ __forceinline__ float act_value(int act, float u)
+// All of a thread's values, the choice of the function outside the loop.
+template <int ACT, int NV> __device__ __forceinline__ void act_values_of(float (*u)[4])
 {
-    if (act == kActCelu) return act_value<kActCelu>(u);
-    if (act == kActGaussian) return act_value<kActGaussian>(u);
-    if (act == kActNormal) return act_value<kActNormal>(u);
-    return act_value<kActSoftplus>(u);
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[k][i] = act_value<ACT>(u[k][i]);
 }
-__device__ __forceinline__ float act_derivative(int act, float u)
+template <int NV> __device__ __forceinline__ void act_values(int act, float (*u)[4])
 {
-    if (act == kActCelu) return act_derivative<kActCelu>(u);
-    if (act == kActGaussian) return act_derivative<kActGaussian>(u);
-    if (act == kActNormal) return act_derivative<kActNormal>(u);
-    return act_derivative<kActSoftplus>(u);
+    if (act == kActCelu) act_values_of<kActCelu, NV>(u);
+    else if (act == kActGaussian) act_values_of<kActGaussian, NV>(u);
+    else if (act == kActNormal) act_values_of<kActNormal, NV>(u);
+    else act_values_of<kActSoftplus, NV>(u);
+}
+template <int ACT, int NV> __device__ __forceinline__ void act_derivatives_of(float (*u)[4])
+{
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[k][i] = act_derivative<ACT>(u[k][i]);
+}
+template <int NV> __device__ __forceinline__ void act_derivatives(int act, float (*u)[4])
+{
+    if (act == kActCelu) act_derivatives_of<kActCelu, NV>(u);
+    else if (act == kActGaussian) act_derivatives_of<kActGaussian, NV>(u);
+    else if (act == kActNormal) act_derivatives_of<kActNormal, NV>(u);
+    else act_derivatives_of<kActSoftplus, NV>(u);
+}
+
+// Smallest and largest value of a block: over the lanes that share it, NaN if one of them has one.
+template <int TEAM> __device__ __forceinline__ void block_extremes(float* low, float* high)
+{
+    if (TEAM >= kWarp) {
+        float l, h;
+        asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(l) : "f"(*low));
+        asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(h) : "f"(*high));
+        *low = l;
+        *high = h;
+    } else {
+#pragma unroll
+        for (int o = TEAM / 2; o > 0; o >>= 1) {
+            *low = min_nan(*low, __shfl_xor_sync(kFull, *low, o));
+            *high = max_nan(*high, __shfl_xor_sync(kFull, *high, o));
+        }
+    }
 }
 
 struct CheckpointParams {
@@ -126,36 +159,39 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
                     low = min_nan(low, z[k][i]);
                     high = max_nan(high, z[k][i]);
                 }
-#pragma unroll
-            for (int o = (TEAM < kWarp ? TEAM : kWarp) / 2; o > 0; o >>= 1) {
-                low = min_nan(low, __shfl_xor_sync(kFull, low, o));
-                high = max_nan(high, __shfl_xor_sync(kFull, high, o));
-            }
+            block_extremes<TEAM>(&low, &high);
             if (!live || col >= w) continue;
             const float spread = __fsub_rn(high, low);
             float step = __fmul_rn(spread, 1.0f / 255.0f);
             const bool finite = spread < __int_as_float(0x7f800000), some = finite && step >= 1e-30f;
             const float inv = some ? __frcp_rn(step) : 0.0f;
             step = some ? step : 0.0f;
+            // rint of 0 .. 255 in one addition: 2^23 + q has its last place at 1, and q in the low bits
             unsigned code = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float q = some && col + i < w ? fminf(rintf(__fmul_rn(__fsub_rn(z[k][i], low), inv)), 255.0f) : 0.0f;
-                code |= (unsigned)q << (8 * i);
+                const float q = __fadd_rn(fminf(__fmul_rn(__fsub_rn(z[k][i], low), inv), 255.0f), 8388608.0f);
+                code |= (some && col + i < w ? __float_as_uint(q) & 255u : 0u) << (8 * i);
             }
             *reinterpret_cast<unsigned*>(p.codes + row * row_bytes + col) = code;
             if (col % kCheckpointBlock == 0)
                 p.blocks[row * row_blocks + col / kCheckpointBlock] = make_float2(finite ? low : __int_as_float(0x7fffffff), step);
-            float g[4], h[4];
             if (NORM) {
+                float g[4], h[4];
                 load_columns(p.gain[e], col, w, p.vec, g);
                 load_columns(p.bias[e], col, w, p.vec, h);
-            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) z[k][i] = act_value(p.act, NORM ? (z[k][i] - mean) * rstd * g[i] + h[i] : z[k][i]);
-            store_columns(p.a + row * w, col, w, p.vec, z[k]);
+                for (int i = 0; i < 4; i++) z[k][i] = (z[k][i] - mean) * rstd * g[i] + h[i];
+            }
         }
-        if (NORM && live && lane == 0) {
+        act_values<NV>(p.act, z);
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            if (col < w) store_columns(p.a + row * w, col, w, p.vec, z[k]);
+        }
+        if (NORM && lane == 0) {
             p.mean[row] = mean;
             p.rstd[row] = rstd;
         }
@@ -187,7 +223,7 @@ __device__ __forceinline__ void load_codes(const unsigned char* codes, const flo
 }
 
 template <int TEAM, int NV, bool NORM>
-__global__ void __launch_bounds__(kNormThreads) checkpoint_activation_grad_kernel(const __grid_constant__ CheckpointGradParams p)
+__global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_activation_grad_kernel(const __grid_constant__ CheckpointGradParams p)
 {
     constexpr int Q = NORM ? 3 : 1;
     __shared__ float scratch[2 * kNormThreads / kWarp];
@@ -200,13 +236,18 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_grad_kerne
     zero_sums_without_rows(p.sums, p.ranges, w);
     if ((int)blockIdx.x >= p.ranges.range_start[kTypes]) return;      // no rows at all: one CTA, for the zeros
     const RowRange range = range_of_cta(p.ranges, blockIdx.x);
-    float gain[NV][4], bias[NV][4], sums[Q][NV][4];
+    // gain and bias in shared memory: in registers they would cost half of the resident warps at 512 columns
+    __shared__ alignas(16) float gain_sh[NORM ? TEAM * NV * 4 : 4], bias_sh[NORM ? TEAM * NV * 4 : 4];
+    if (NORM) {
+        for (int c = threadIdx.x; c < TEAM * NV * 4; c += kNormThreads) {
+            gain_sh[c] = c < w ? p.gain[range.element][c] : 0.0f;
+            bias_sh[c] = c < w ? p.bias[range.element][c] : 0.0f;
+        }
+        __syncthreads();
+    }
+    float sums[Q][NV][4];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        if (NORM) {
-            load_columns(p.gain[range.element], 4 * (lane + k * TEAM), w, p.vec, gain[k]);
-            load_columns(p.bias[range.element], 4 * (lane + k * TEAM), w, p.vec, bias[k]);
-        }
 #pragma unroll
         for (int q = 0; q < Q; q++)
 #pragma unroll
@@ -228,17 +269,23 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_grad_kerne
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int col = 4 * (lane + k * TEAM);
+                float g[4], h[4], d[1][4];
+                load4(gain_sh + col, g);
+                load4(bias_sh + col, h);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const bool in = live && col + i < w;
-                    const float xhat = in ? (kept[k][i] - mean) * rstd : 0.0f;
-                    const float du = in ? up[k][i] * act_derivative(p.act, xhat * gain[k][i] + bias[k][i]) : 0.0f;
-                    kept[k][i] = xhat;
-                    sums[Q - 2][k][i] += du * xhat;
+                    kept[k][i] = live && col + i < w ? (kept[k][i] - mean) * rstd : 0.0f;
+                    d[0][i] = kept[k][i] * g[i] + h[i];
+                }
+                act_derivatives<1>(p.act, d);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float du = up[k][i] * d[0][i];      // up is zero where there is no value
+                    sums[Q - 2][k][i] += du * kept[k][i];
                     sums[Q - 1][k][i] += du;
-                    up[k][i] = du * gain[k][i];
+                    up[k][i] = du * g[i];
                     sum[0] += up[k][i];
-                    sum[1] += up[k][i] * xhat;
+                    sum[1] += up[k][i] * kept[k][i];
                 }
             }
             team_sum<TEAM, 2>(sum, scratch);
@@ -249,10 +296,11 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_grad_kerne
 #pragma unroll
                 for (int i = 0; i < 4; i++) up[k][i] = rstd * (up[k][i] - sum[0] - kept[k][i] * sum[1]);
         } else {
+            act_derivatives<NV>(p.act, kept);
 #pragma unroll
             for (int k = 0; k < NV; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) up[k][i] *= act_derivative(p.act, kept[k][i]);
+                for (int i = 0; i < 4; i++) up[k][i] *= kept[k][i];
         }
         if (!live) continue;
 #pragma unroll
