@@ -41,10 +41,22 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // The activation functions on the special function unit's exponential (2^-22 of its value; the argument's rounding adds
 // |x| 2^-24): a few 1e-7 of max(1, |a|), in a quarter of the instructions of expf and log1pf, and without a branch: celu as
 // "u or 0.1 (exp(10 u) - 1)" was compiled to one, and 32 values of a thread took 5000 clocks instead of 700.
+__device__ __forceinline__ float fast_exp(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+__device__ __forceinline__ float fast_reciprocal(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 // log(1 + e) for e in [0, 1] = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series: what is cut off is below 2e-8 of it.
 __device__ __forceinline__ float log1p_unit(float e)
 {
-    const float s = __fdividef(e, 2.0f + e), t = s * s;
+    const float s = e * fast_reciprocal(2.0f + e), t = s * s;
     float p = 1.0f / 13.0f;
     p = fmaf(p, t, 1.0f / 11.0f);
     p = fmaf(p, t, 1.0f / 9.0f);
@@ -55,17 +67,17 @@ __device__ __forceinline__ float log1p_unit(float e)
 }
 template <int ACT> __device__ __forceinline__ float act_value(float u)
 {
-    if (ACT == kActCelu) return fmaxf(u, 0.0f) + fmaf(0.1f, __expf(min_nan(10.0f * u, 0.0f)), -0.1f);
-    if (ACT == kActGaussian) return __expf(-u * u);
-    if (ACT == kActNormal) return __expf(-0.5f * u * u);
-    return fmaxf(u, 0.0f) + log1p_unit(__expf(-fabsf(u))) - 0.69314718056f;
+    if (ACT == kActCelu) return fmaxf(u, 0.0f) + fmaf(0.1f, fast_exp(min_nan(10.0f * u, 0.0f)), -0.1f);
+    if (ACT == kActGaussian) return fast_exp(-u * u);
+    if (ACT == kActNormal) return fast_exp(-0.5f * u * u);
+    return fmaxf(u, 0.0f) + log1p_unit(fast_exp(-fabsf(u))) - 0.69314718056f;
 }
 template <int ACT> __device__ __forceinline__ float act_derivative(float u)
 {
-    if (ACT == kActCelu) return __expf(min_nan(10.0f * u, 0.0f));
-    if (ACT == kActGaussian) return -2.0f * u * __expf(-u * u);
-    if (ACT == kActNormal) return -u * __expf(-0.5f * u * u);
-    return __fdividef(1.0f, 1.0f + __expf(-u));
+    if (ACT == kActCelu) return fast_exp(min_nan(10.0f * u, 0.0f));
+    if (ACT == kActGaussian) return -2.0f * u * fast_exp(-u * u);
+    if (ACT == kActNormal) return -u * fast_exp(-0.5f * u * u);
+    return fast_reciprocal(1.0f + fast_exp(-u));
 }
 // All of a thread's values, the choice of the function outside the loop.
 template <int ACT, int NV> __device__ __forceinline__ void act_values_of(float (*u)[4])
@@ -125,14 +137,15 @@ struct CheckpointParams {
     float2* blocks;            // [n][checkpoint_blocks]: base, step
     float *mean, *rstd;
     RowGroups groups;
-    int width, vec, act;
+    int width, act;
     float inv_w, eps;
 };
 
-template <int TEAM, int NV, bool NORM>
+template <int TEAM, int NV, bool NORM, bool VEC>
 __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(const __grid_constant__ CheckpointParams p)
 {
-    __shared__ float scratch[kNormThreads / kWarp];
+    __shared__ float scratch_sh[4 * kNormThreads / kWarp];
+    TeamScratch<float> scratch = {scratch_sh, 0};
     constexpr int teams = kNormThreads / TEAM;
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
     const int row_bytes = checkpoint_row_bytes(w), row_blocks = checkpoint_blocks(w);
@@ -145,20 +158,25 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
         float z[NV][4];
 #pragma unroll
         for (int k = 0; k < NV; k++)
-            load_columns(p.z + row * p.z_stride, 4 * (lane + k * TEAM), w, p.vec, z[k]);
+            load_columns<VEC>(p.z + row * p.z_stride, 4 * (lane + k * TEAM), w, z[k]);
         float mean = 0.0f, rstd = 1.0f;
-        if (NORM) row_statistics<TEAM, NV>(z, lane, w, p.inv_w, p.eps, scratch, &mean, &rstd);
+        if (NORM) row_statistics<TEAM, NV, VEC>(z, lane, w, p.inv_w, p.eps, scratch, &mean, &rstd);
         const int e = element_of_row(p.groups, row);
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
             float low = __int_as_float(0x7f800000), high = -low;
+            if (VEC && col < w) {
+                low = min_nan(min_nan(z[k][0], z[k][1]), min_nan(z[k][2], z[k][3]));
+                high = max_nan(max_nan(z[k][0], z[k][1]), max_nan(z[k][2], z[k][3]));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (col + i < w) {
-                    low = min_nan(low, z[k][i]);
-                    high = max_nan(high, z[k][i]);
-                }
+                for (int i = 0; i < 4; i++)
+                    if (col + i < w) {
+                        low = min_nan(low, z[k][i]);
+                        high = max_nan(high, z[k][i]);
+                    }
+            }
             block_extremes<TEAM>(&low, &high);
             if (!live || col >= w) continue;
             const float spread = __fsub_rn(high, low);
@@ -166,20 +184,19 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
             const bool finite = spread < __int_as_float(0x7f800000), some = finite && step >= 1e-30f;
             const float inv = some ? __frcp_rn(step) : 0.0f;
             step = some ? step : 0.0f;
-            // rint of 0 .. 255 in one addition: 2^23 + q has its last place at 1, and q in the low bits
-            unsigned code = 0;
+            // rint of 0 .. 255 in one addition: 2^23 + q has its last place at 1, and q in the low bits.  Nothing is above
+            // 255: (max - base) (1 / step) is 255 but for four roundings.
+            unsigned q[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float q = __fadd_rn(fminf(__fmul_rn(__fsub_rn(z[k][i], low), inv), 255.0f), 8388608.0f);
-                code |= (some && col + i < w ? __float_as_uint(q) & 255u : 0u) << (8 * i);
-            }
+            for (int i = 0; i < 4; i++) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(z[k][i], low), inv), 8388608.0f));
+            const unsigned code = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
             *reinterpret_cast<unsigned*>(p.codes + row * row_bytes + col) = code;
             if (col % kCheckpointBlock == 0)
                 p.blocks[row * row_blocks + col / kCheckpointBlock] = make_float2(finite ? low : __int_as_float(0x7fffffff), step);
             if (NORM) {
                 float g[4], h[4];
-                load_columns(p.gain[e], col, w, p.vec, g);
-                load_columns(p.bias[e], col, w, p.vec, h);
+                load_columns<VEC>(p.gain[e], col, w, g);
+                load_columns<VEC>(p.bias[e], col, w, h);
 #pragma unroll
                 for (int i = 0; i < 4; i++) z[k][i] = (z[k][i] - mean) * rstd * g[i] + h[i];
             }
@@ -189,7 +206,7 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
-            if (col < w) store_columns(p.a + row * w, col, w, p.vec, z[k]);
+            if (col < w) store_columns<VEC>(p.a + row * w, col, w, z[k]);
         }
         if (NORM && lane == 0) {
             p.mean[row] = mean;
@@ -209,24 +226,16 @@ struct CheckpointGradParams {
     float* grad_z;
     ColumnSums<float, 3> sums;      // of dz, and with a gain of its gradient and the bias'
     RowRanges ranges;
-    int width, vec, act;
+    int width, act;
     float inv_w;
 };
 
-// The four values at column col that the codes of a row stand for.
-__device__ __forceinline__ void load_codes(const unsigned char* codes, const float2* blocks, int col, int w, float* z)
-{
-    const unsigned code = col < w ? *reinterpret_cast<const unsigned*>(codes + col) : 0u;
-    const float2 b = col < w ? blocks[col / kCheckpointBlock] : make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < 4; i++) z[i] = fmaf((float)((code >> (8 * i)) & 255u), b.y, b.x);
-}
-
-template <int TEAM, int NV, bool NORM>
+template <int TEAM, int NV, bool NORM, bool VEC>
 __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_activation_grad_kernel(const __grid_constant__ CheckpointGradParams p)
 {
     constexpr int Q = NORM ? 3 : 1;
-    __shared__ float scratch[2 * kNormThreads / kWarp];
+    __shared__ float scratch_sh[4 * kNormThreads / kWarp];
+    TeamScratch<float> scratch = {scratch_sh, 0};
     __shared__ alignas(16) float tile[TEAM == kNormThreads ? 4 : kNormThreads * NV * 4];
     constexpr int teams = kNormThreads / TEAM;
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
@@ -256,15 +265,27 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
     for (long long first = range.first; first < range.end; first += teams) {
         const bool live = first + team < range.end;
         const long long row = live ? first + team : first;
-        float kept[NV][4], up[NV][4];
+        // everything a row needs is asked for before any of it is used
+        float kept[NV][4], up[NV][4], mean = 0.0f, rstd = 0.0f;
+        unsigned code[NV];
+        float2 block[NV];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
-            load_codes(p.codes + row * row_bytes, p.blocks + row * row_blocks, col, live ? w : 0, kept[k]);
-            load_columns(p.grad_a + row * p.grad_stride, col, live ? w : 0, p.vec, up[k]);
+            const bool in = live && col < w;
+            code[k] = in ? *reinterpret_cast<const unsigned*>(p.codes + row * row_bytes + col) : 0u;
+            block[k] = in ? p.blocks[row * row_blocks + col / kCheckpointBlock] : make_float2(0.0f, 0.0f);
+            load_columns<VEC>(p.grad_a + row * p.grad_stride, col, live ? w : 0, up[k]);
         }
+        if (NORM) {
+            mean = p.mean[row];
+            rstd = p.rstd[row];
+        }
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) kept[k][i] = fmaf((float)((code[k] >> (8 * i)) & 255u), block[k].y, block[k].x);
         if constexpr (NORM) {
-            const float mean = p.mean[row], rstd = p.rstd[row];
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < NV; k++) {
@@ -274,7 +295,7 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
                 load4(bias_sh + col, h);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    kept[k][i] = live && col + i < w ? (kept[k][i] - mean) * rstd : 0.0f;
+                    kept[k][i] = live && column_in<VEC>(col, i, w) ? (kept[k][i] - mean) * rstd : 0.0f;
                     d[0][i] = kept[k][i] * g[i] + h[i];
                 }
                 act_derivatives<1>(p.act, d);
@@ -309,7 +330,7 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
             if (col >= w) break;
 #pragma unroll
             for (int i = 0; i < 4; i++) sums[0][k][i] += up[k][i];
-            store_columns(p.grad_z + row * w, col, w, p.vec, up[k]);
+            store_columns<VEC>(p.grad_z + row * w, col, w, up[k]);
         }
     }
 #pragma unroll

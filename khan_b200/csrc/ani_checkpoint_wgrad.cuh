@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum
 #pragma unroll 4
     for (int k = begin; k < end; k++) {
         float v[4];
-        load_columns(p.partial + (size_t)(first + k) * size, at, size, vec, v);
+        if (vec) load_columns<true>(p.partial + (size_t)(first + k) * size, at, size, v);
+        else load_columns<false>(p.partial + (size_t)(first + k) * size, at, size, v);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[i] += v[i];
     }

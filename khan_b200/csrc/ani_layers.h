@@ -46,31 +46,52 @@ bool one_range_each(const RowRanges& r)
     return true;
 }
 
-// The team and the columns per thread for a row of `width` values.
-template <typename F> cudaError_t with_team(int width, F f)
+// The team and the columns per thread for a row of `width` values.  In the activations' backward pass and in double precision
+// a thread holds more than twice as much per column: HEAVY, more threads to a row.
+template <bool HEAVY, typename F> cudaError_t with_team(int width, bool vec, F f)
 {
-#define ANI_TEAM(TEAM, NV) f(std::integral_constant<int, TEAM>(), std::integral_constant<int, NV>())
+#define ANI_TEAM(TEAM, NV)                                                                                            \
+    (vec ? f(std::integral_constant<int, TEAM>(), std::integral_constant<int, NV>(), std::true_type())               \
+         : f(std::integral_constant<int, TEAM>(), std::integral_constant<int, NV>(), std::false_type()))
     const int quads = (width + 3) / 4;
     if (quads <= 8) return ANI_TEAM(8, 1);
     if (quads <= 16) return ANI_TEAM(16, 1);
     if (quads <= 32) return ANI_TEAM(32, 1);
-    if (quads <= 64) return ANI_TEAM(32, 2);
-    if (quads <= 128) return ANI_TEAM(32, 4);
-    if (quads <= 256) return ANI_TEAM(256, 1);
+    if constexpr (HEAVY) {
+        if (quads <= 64) return ANI_TEAM(64, 1);
+        if (quads <= 128) return ANI_TEAM(64, 2);
+        if (quads <= 256) return ANI_TEAM(128, 2);
+    } else {
+        if (quads <= 64) return ANI_TEAM(32, 2);
+        if (quads <= 128) return ANI_TEAM(32, 4);
+        if (quads <= 256) return ANI_TEAM(256, 1);
+    }
     if (quads <= 512) return ANI_TEAM(256, 2);
     return ANI_TEAM(256, 4);
 #undef ANI_TEAM
 }
-int rows_at_once(int width)
+template <bool HEAVY> int rows_at_once(int width)
 {
-    const int quads = (width + 3) / 4;
-    return quads <= 8 ? 32 : quads <= 16 ? 16 : quads <= 128 ? 8 : 1;
+    int rows = 1;
+    with_team<HEAVY>(width, true, [&](auto team, auto, auto) {
+        rows = kNormThreads / team();
+        return cudaSuccess;
+    });
+    return rows;
 }
 
-// Ranges of the launches with sums over rows.
-RowRanges sum_ranges(const int* acs, int width)
+// Whether the launch with `sums` sums of values of `size` bytes takes the larger teams.
+constexpr bool heavy_sums(int sums, size_t size) { return sums > 2 || size > 4; }
+// Ranges of the launches with sums over rows: as many CTAs as are resident at once (their registers, 40 to 224 a thread).
+RowRanges sum_ranges(const int* acs, int width, int sums, size_t size)
 {
-    return row_ranges(acs, 2 * kSms, rows_at_once(width), 4 * rows_at_once(width));
+    const int quads = (width + 3) / 4;
+    const bool heavy = heavy_sums(sums, size);
+    const int rows = heavy ? rows_at_once<true>(width) : rows_at_once<false>(width);
+    int per_sm = 4;
+    if (heavy && quads > 32) per_sm = size > 4 ? (quads > 512 ? 1 : 2) : (quads > 512 ? 2 : 3);
+    if (!heavy && quads > 32) per_sm = quads <= 64 ? 3 : quads <= 128 ? 2 : quads <= 256 ? 6 : quads <= 512 ? 4 : 2;
+    return row_ranges(acs, per_sm * kSms, rows, 4 * rows);
 }
 size_t sums_workspace(const RowRanges& r, int sums, int width, size_t size)
 {
@@ -123,10 +144,10 @@ int layer_norm(const T* x, long long x_stride, const T* const* gain, const T* co
     if (int rc = take_pointers(bias, acs, p.bias, &vec)) return rc;
     p.x = x; p.x_stride = x_stride; p.y = y; p.mean = mean; p.rstd = rstd;
     p.groups = row_groups(acs);
-    p.width = width; p.vec = vec; p.inv_w = T(1) / T(width); p.eps = T(eps);
-    const int grid = rows_grid(n, rows_at_once(width));
-    ANI_CUDA(with_team(width, [&](auto team, auto nv) {
-        return launch_chain(layer_norm_kernel<T, team(), nv()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
+    p.width = width; p.inv_w = T(1) / T(width); p.eps = T(eps);
+    const int grid = rows_grid(n, rows_at_once<false>(width));
+    ANI_CUDA(with_team<false>(width, vec, [&](auto team, auto nv, auto aligned) {
+        return launch_chain(layer_norm_kernel<T, team(), nv(), aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return ANI_OK;
 }
@@ -145,14 +166,14 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
     if (int rc = take_pointers(gain, acs, p.gain, &vec)) return rc;
     if (int rc = take_pointers(grad_gain, acs, p.sums.out[0])) return rc;
     if (int rc = take_pointers(grad_bias, acs, p.sums.out[1])) return rc;
-    p.ranges = sum_ranges(acs, width);
+    p.ranges = sum_ranges(acs, width, 2, sizeof(T));
     if (sums_workspace(p.ranges, 2, width, sizeof(T)) && !workspace) return ANI_ERR_NULL_POINTER;
     p.sums.partial = static_cast<T*>(workspace);
     p.grad_y = grad_y; p.grad_stride = grad_stride; p.x = x; p.x_stride = x_stride; p.mean = mean; p.rstd = rstd;
-    p.grad_x = grad_x; p.width = width; p.vec = vec; p.inv_w = T(1) / T(width);
+    p.grad_x = grad_x; p.width = width; p.inv_w = T(1) / T(width);
     const int grid = std::max(1, p.ranges.range_start[kTypes]);
-    ANI_CUDA(with_team(width, [&](auto team, auto nv) {
-        return launch_chain(layer_norm_grad_kernel<T, team(), nv()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
+    ANI_CUDA(with_team<heavy_sums(2, sizeof(T))>(width, vec, [&](auto team, auto nv, auto aligned) {
+        return launch_chain(layer_norm_grad_kernel<T, team(), nv(), aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return column_sums_launch(p.sums, p.ranges, width, (cudaStream_t)stream);
 }
@@ -227,7 +248,7 @@ size_t ani_layer_sums_workspace_bytes(int width, const int* acs_host, int sums, 
 {
     long long n = 0;
     if (check_layer(acs_host, width, &n) || sums < 0 || value_bytes < 0) return 0;
-    return sums_workspace(sum_ranges(acs_host, width), sums, width, (size_t)value_bytes);
+    return sums_workspace(sum_ranges(acs_host, width, sums, (size_t)value_bytes), sums, width, (size_t)value_bytes);
 }
 
 int ani_checkpoint_row_bytes(int width) { return width < 1 || width > kNormMaxWidth ? ANI_ERR_BAD_SIZE : checkpoint_row_bytes(width); }
@@ -252,11 +273,11 @@ int ani_checkpoint_activation_f32(const float* z, long long z_stride, const floa
     if (!aligned16({codes}) || (reinterpret_cast<uintptr_t>(blocks) & 7)) return ANI_ERR_MISALIGNED;
     p.z = z; p.z_stride = z_stride; p.a = a; p.codes = codes; p.blocks = reinterpret_cast<float2*>(blocks);
     p.mean = mean; p.rstd = rstd; p.groups = row_groups(acs_host);
-    p.width = width; p.vec = vec; p.act = activation; p.inv_w = 1.0f / (float)width; p.eps = (float)eps;
-    const int grid = rows_grid(n, rows_at_once(width));
-    ANI_CUDA(with_team(width, [&](auto team, auto nv) {
-        return gain_host ? launch_chain(checkpoint_activation_kernel<team(), nv(), true>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p)
-                         : launch_chain(checkpoint_activation_kernel<team(), nv(), false>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
+    p.width = width; p.act = activation; p.inv_w = 1.0f / (float)width; p.eps = (float)eps;
+    const int grid = rows_grid(n, rows_at_once<false>(width));
+    ANI_CUDA(with_team<false>(width, vec, [&](auto team, auto nv, auto aligned) {
+        return gain_host ? launch_chain(checkpoint_activation_kernel<team(), nv(), true, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p)
+                         : launch_chain(checkpoint_activation_kernel<team(), nv(), false, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return ANI_OK;
 }
@@ -282,16 +303,16 @@ int ani_checkpoint_activation_grad_f32(const unsigned char* codes, const float* 
         if (int rc = take_pointers(grad_bias_host, acs_host, p.sums.out[2])) return rc;
     }
     if (!aligned16({codes}) || (reinterpret_cast<uintptr_t>(blocks) & 7)) return ANI_ERR_MISALIGNED;
-    p.ranges = sum_ranges(acs_host, width);
+    p.ranges = sum_ranges(acs_host, width, 3, sizeof(float));
     if (sums_workspace(p.ranges, 3, width, sizeof(float)) && !workspace) return ANI_ERR_NULL_POINTER;
     p.sums.partial = static_cast<float*>(workspace);
     p.codes = codes; p.blocks = reinterpret_cast<const float2*>(blocks); p.mean = mean; p.rstd = rstd;
     p.grad_a = grad_a; p.grad_stride = grad_stride; p.grad_z = grad_z;
-    p.width = width; p.vec = vec; p.act = activation; p.inv_w = 1.0f / (float)width;
+    p.width = width; p.act = activation; p.inv_w = 1.0f / (float)width;
     const int grid = std::max(1, p.ranges.range_start[kTypes]);
-    ANI_CUDA(with_team(width, [&](auto team, auto nv) {
-        return gain_host ? launch_chain(checkpoint_activation_grad_kernel<team(), nv(), true>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p)
-                         : launch_chain(checkpoint_activation_grad_kernel<team(), nv(), false>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
+    ANI_CUDA(with_team<true>(width, vec, [&](auto team, auto nv, auto aligned) {
+        return gain_host ? launch_chain(checkpoint_activation_grad_kernel<team(), nv(), true, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p)
+                         : launch_chain(checkpoint_activation_grad_kernel<team(), nv(), false, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return column_sums_launch(p.sums, p.ranges, width, (cudaStream_t)stream);
 }

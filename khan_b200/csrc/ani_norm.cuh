@@ -5,7 +5,7 @@
 //   mean = sum x / w,  rstd = 1 / sqrt(sum (x - mean)^2 / w + eps),  xhat = (x - mean) rstd,  y = gain xhat + bias;
 //   g = gain dy:  dx = rstd (g - sum g / w - xhat sum(g xhat) / w),  dgain = sum over rows dy xhat,  dbias = sum over rows dy.
 //
-// A row belongs to a TEAM of threads (8, 16 or 32 lanes of a warp, or a CTA of 256), which keeps it in registers: thread l
+// A row belongs to a TEAM of threads (8, 16 or 32 lanes of a warp, or 2, 4 or 8 warps), which keeps it in registers: thread l
 // holds the NV groups of four consecutive columns 4 (l + k TEAM), so that the row is read once and the variance is the
 // two-pass one (a mean far from zero costs nothing).  Columns are four to a thread whether or not the rows are 16-byte
 // aligned; only the load instruction differs.  All sums are held in the type of the rows: 32 bits for float.
@@ -53,26 +53,34 @@ __device__ __forceinline__ RowRange range_of_cta(const RowRanges& r, int cta)
     return out;
 }
 
-// Four consecutive columns of a row; columns >= w read as zero and are not written.
-template <typename T> __device__ __forceinline__ void load_columns(const T* row, int col, int w, bool vec, T* v)
+// Four consecutive columns of a row; columns >= w read as zero and are not written.  VEC: w is a multiple of four and the
+// columns are one 16-byte access (two in double).
+template <bool VEC, typename T> __device__ __forceinline__ void load_columns(const T* row, int col, int w, T* v)
 {
-    if (vec && col + 4 <= w) {
-        load4(row + col, v);
+    if (VEC) {
+        if (col < w) {
+            load4(row + col, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = T(0);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = col + i < w ? row[col + i] : T(0);
     }
 }
+// Whether column i of the four is inside the row (with VEC all are, or none).
+template <bool VEC> __device__ __forceinline__ bool column_in(int col, int i, int w) { return VEC ? col < w : col + i < w; }
 __device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void store4(double* p, const double* v)
 {
     *reinterpret_cast<double2*>(p) = make_double2(v[0], v[1]);
     *reinterpret_cast<double2*>(p + 2) = make_double2(v[2], v[3]);
 }
-template <typename T> __device__ __forceinline__ void store_columns(T* row, int col, int w, bool vec, const T* v)
+template <bool VEC, typename T> __device__ __forceinline__ void store_columns(T* row, int col, int w, const T* v)
 {
-    if (vec && col + 4 <= w) {
-        store4(row + col, v);
+    if (VEC) {
+        if (col < w) store4(row + col, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -80,24 +88,49 @@ template <typename T> __device__ __forceinline__ void store_columns(T* row, int 
     }
 }
 
-// Sums over a team, the same value in all of its threads.  Every thread of the CTA takes part.
-template <int TEAM, int N, typename T> __device__ __forceinline__ void team_sum(T* v, T* scratch)
+// Barrier of the threads of a team of several warps.  (With the number in a register the compiler sets all sixteen barriers
+// of a CTA aside.)
+template <int TEAM> __device__ __forceinline__ void team_sync()
+{
+    if (TEAM == kNormThreads) {
+        __syncthreads();
+    } else {
+        const int team = threadIdx.x / TEAM;
+        if (team == 0) asm volatile("bar.sync 1, %0;" ::"n"(TEAM) : "memory");
+        else if (team == 1) asm volatile("bar.sync 2, %0;" ::"n"(TEAM) : "memory");
+        else if (team == 2) asm volatile("bar.sync 3, %0;" ::"n"(TEAM) : "memory");
+        else asm volatile("bar.sync 4, %0;" ::"n"(TEAM) : "memory");
+    }
+}
+static_assert(kNormThreads / 64 == 4, "teams of two warps or more: four at most");
+// Where the warps of a team meet; two places in turn, so that a sum needs one barrier.
+template <typename T> struct TeamScratch {
+    T* values;      // [2][2 * warps of the CTA]
+    int which;
+    __device__ __forceinline__ T* next()
+    {
+        which ^= 1;
+        return values + which * (2 * kNormThreads / kWarp);
+    }
+};
+// Sums over a team, the same value in all of its threads; N <= 2.  Every thread of the CTA takes part.
+template <int TEAM, int N, typename T> __device__ __forceinline__ void team_sum(T* v, TeamScratch<T>& scratch)
 {
 #pragma unroll
     for (int o = (TEAM < kWarp ? TEAM : kWarp) / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(kFull, v[i], o);
     if (TEAM > kWarp) {
-        __syncthreads();      // the values of the sum before have been read
+        T* place = scratch.next() + threadIdx.x / TEAM * (TEAM / kWarp) * N;
         if (lane_id() == 0)
 #pragma unroll
-            for (int i = 0; i < N; i++) scratch[warp_id() * N + i] = v[i];
-        __syncthreads();
+            for (int i = 0; i < N; i++) place[warp_id() % (TEAM / kWarp) * N + i] = v[i];
+        team_sync<TEAM>();
 #pragma unroll
         for (int i = 0; i < N; i++) {
             T s = T(0);
 #pragma unroll
-            for (int k = 0; k < TEAM / kWarp; k++) s += scratch[k * N + i];
+            for (int k = 0; k < TEAM / kWarp; k++) s += place[k * N + i];
             v[i] = s;
         }
     }
@@ -107,8 +140,9 @@ __device__ __forceinline__ float rsqrt_full(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double rsqrt_full(double v) { return 1.0 / sqrt(v); }
 
 // mean and 1 / sqrt(variance + eps) of the row that the team holds in x.
-template <int TEAM, int NV, typename T>
-__device__ __forceinline__ void row_statistics(const T (*x)[4], int lane, int w, T inv_w, T eps, T* scratch, T* mean, T* rstd)
+template <int TEAM, int NV, bool VEC, typename T>
+__device__ __forceinline__ void row_statistics(const T (*x)[4], int lane, int w, T inv_w, T eps, TeamScratch<T>& scratch,
+                                               T* mean, T* rstd)
 {
     T s = T(0);
 #pragma unroll
@@ -121,7 +155,7 @@ __device__ __forceinline__ void row_statistics(const T (*x)[4], int lane, int w,
         const int col = 4 * (lane + k * TEAM);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const T d = col + i < w ? x[k][i] - m : T(0);
+            const T d = column_in<VEC>(col, i, w) ? x[k][i] - m : T(0);
             q += d * d;
         }
     }
@@ -139,7 +173,7 @@ __device__ __forceinline__ void store_column_sums(const T (*v)[4], T* tile, T* o
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     if (TEAM == kNormThreads) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) store_columns(out, 4 * (lane + k * TEAM), w, false, v[k]);
+        for (int k = 0; k < NV; k++) store_columns<false>(out, 4 * (lane + k * TEAM), w, v[k]);
         return;
     }
     __syncthreads();      // the tile of the sums before has been read
@@ -209,14 +243,15 @@ template <typename T> struct LayerNormParams {
     const T* bias[kTypes];
     T *y, *mean, *rstd;
     RowGroups groups;
-    int width, vec;
+    int width;
     T inv_w, eps;
 };
 
-template <typename T, int TEAM, int NV>
+template <typename T, int TEAM, int NV, bool VEC>
 __global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const __grid_constant__ LayerNormParams<T> p)
 {
-    __shared__ T scratch[kNormThreads / kWarp];
+    __shared__ T scratch_sh[4 * kNormThreads / kWarp];
+    TeamScratch<T> scratch = {scratch_sh, 0};
     constexpr int teams = kNormThreads / TEAM;
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const long long n = p.groups.start[kTypes];
@@ -228,9 +263,9 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const __grid_c
         T x[NV][4];
 #pragma unroll
         for (int k = 0; k < NV; k++)
-            load_columns(p.x + (live ? row : 0) * p.x_stride, 4 * (lane + k * TEAM), live ? p.width : 0, p.vec, x[k]);
+            load_columns<VEC>(p.x + (live ? row : 0) * p.x_stride, 4 * (lane + k * TEAM), live ? p.width : 0, x[k]);
         T mean, rstd;
-        row_statistics<TEAM, NV>(x, lane, p.width, p.inv_w, p.eps, scratch, &mean, &rstd);
+        row_statistics<TEAM, NV, VEC>(x, lane, p.width, p.inv_w, p.eps, scratch, &mean, &rstd);
         if (!live) continue;      // the teams of a CTA of 256 are one, and live
         const int e = element_of_row(p.groups, row);
         const T *gain = p.gain[e], *bias = p.bias[e];
@@ -240,11 +275,11 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const __grid_c
             const int col = 4 * (lane + k * TEAM);
             if (col >= p.width) break;
             T g[4], h[4];
-            load_columns(gain, col, p.width, p.vec, g);
-            load_columns(bias, col, p.width, p.vec, h);
+            load_columns<VEC>(gain, col, p.width, g);
+            load_columns<VEC>(bias, col, p.width, h);
 #pragma unroll
             for (int i = 0; i < 4; i++) g[i] = (x[k][i] - mean) * rstd * g[i] + h[i];
-            store_columns(y, col, p.width, p.vec, g);
+            store_columns<VEC>(y, col, p.width, g);
         }
         if (lane == 0) {
             p.mean[row] = mean;
@@ -263,14 +298,15 @@ template <typename T> struct LayerNormGradParams {
     T* grad_x;
     ColumnSums<T, 2> sums;      // gain, bias
     RowRanges ranges;
-    int width, vec;
+    int width;
     T inv_w;
 };
 
-template <typename T, int TEAM, int NV>
+template <typename T, int TEAM, int NV, bool VEC>
 __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __grid_constant__ LayerNormGradParams<T> p)
 {
-    __shared__ T scratch[2 * kNormThreads / kWarp];
+    __shared__ T scratch_sh[4 * kNormThreads / kWarp];
+    TeamScratch<T> scratch = {scratch_sh, 0};
     __shared__ alignas(16) T tile[TEAM == kNormThreads ? 4 : kNormThreads * NV * 4];
     constexpr int teams = kNormThreads / TEAM;
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, w = p.width;
@@ -282,7 +318,7 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __g
     T gain[NV][4], dgain[NV][4], dbias[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        load_columns(p.gain[range.element], 4 * (lane + k * TEAM), w, p.vec, gain[k]);
+        load_columns<VEC>(p.gain[range.element], 4 * (lane + k * TEAM), w, gain[k]);
 #pragma unroll
         for (int i = 0; i < 4; i++) dgain[k][i] = dbias[k][i] = T(0);
     }
@@ -294,8 +330,8 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __g
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
-            load_columns(p.x + row * p.x_stride, col, live ? w : 0, p.vec, xhat[k]);
-            load_columns(p.grad_y + row * p.grad_stride, col, live ? w : 0, p.vec, up[k]);
+            load_columns<VEC>(p.x + row * p.x_stride, col, live ? w : 0, xhat[k]);
+            load_columns<VEC>(p.grad_y + row * p.grad_stride, col, live ? w : 0, up[k]);
         }
         T sum[2] = {T(0), T(0)};
 #pragma unroll
@@ -303,7 +339,7 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __g
             const int col = 4 * (lane + k * TEAM);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                xhat[k][i] = live && col + i < w ? (xhat[k][i] - mean) * rstd : T(0);
+                xhat[k][i] = live && column_in<VEC>(col, i, w) ? (xhat[k][i] - mean) * rstd : T(0);
                 dgain[k][i] += up[k][i] * xhat[k][i];
                 dbias[k][i] += up[k][i];
                 up[k][i] *= gain[k][i];
@@ -321,7 +357,7 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __g
             if (col >= w) break;
 #pragma unroll
             for (int i = 0; i < 4; i++) up[k][i] = rstd * (up[k][i] - sum[0] - xhat[k][i] * sum[1]);
-            store_columns(p.grad_x + row * w, col, w, p.vec, up[k]);
+            store_columns<VEC>(p.grad_x + row * w, col, w, up[k]);
         }
     }
     store_column_sums<TEAM, NV>(dgain, tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, 0, w), w);
