@@ -41,10 +41,11 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // The activation functions on the special function unit's exponential (2^-22 of its value; the argument's rounding adds
 // |x| 2^-24): a few 1e-7 of max(1, |a|), in a quarter of the instructions of expf and log1pf, and without a branch: celu as
 // "u or 0.1 (exp(10 u) - 1)" was compiled to one, and 32 values of a thread took 5000 clocks instead of 700.
-__device__ __forceinline__ float fast_exp(float x)
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float fast_exp2(float x)
 {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float fast_reciprocal(float x)
@@ -67,17 +68,17 @@ __device__ __forceinline__ float log1p_unit(float e)
 }
 template <int ACT> __device__ __forceinline__ float act_value(float u)
 {
-    if (ACT == kActCelu) return fmaxf(u, 0.0f) + fmaf(0.1f, fast_exp(min_nan(10.0f * u, 0.0f)), -0.1f);
-    if (ACT == kActGaussian) return fast_exp(-u * u);
-    if (ACT == kActNormal) return fast_exp(-0.5f * u * u);
-    return fmaxf(u, 0.0f) + log1p_unit(fast_exp(-fabsf(u))) - 0.69314718056f;
+    if (ACT == kActCelu) return fmaxf(u, 0.0f) + fmaf(0.1f, fast_exp2(min_nan(10.0f * kLog2E * u, 0.0f)), -0.1f);
+    if (ACT == kActGaussian) return fast_exp2(-kLog2E * u * u);
+    if (ACT == kActNormal) return fast_exp2(-0.5f * kLog2E * u * u);
+    return fmaxf(u, 0.0f) + log1p_unit(fast_exp2(-kLog2E * fabsf(u))) - 0.69314718056f;
 }
 template <int ACT> __device__ __forceinline__ float act_derivative(float u)
 {
-    if (ACT == kActCelu) return fast_exp(min_nan(10.0f * u, 0.0f));
-    if (ACT == kActGaussian) return -2.0f * u * fast_exp(-u * u);
-    if (ACT == kActNormal) return -u * fast_exp(-0.5f * u * u);
-    return fast_reciprocal(1.0f + fast_exp(-u));
+    if (ACT == kActCelu) return fast_exp2(min_nan(10.0f * kLog2E * u, 0.0f));
+    if (ACT == kActGaussian) return -2.0f * u * fast_exp2(-kLog2E * u * u);
+    if (ACT == kActNormal) return -u * fast_exp2(-0.5f * kLog2E * u * u);
+    return fast_reciprocal(1.0f + fast_exp2(-kLog2E * u));
 }
 // All of a thread's values, the choice of the function outside the loop.
 template <int ACT, int NV> __device__ __forceinline__ void act_values_of(float (*u)[4])
@@ -262,25 +263,44 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
 #pragma unroll
             for (int i = 0; i < 4; i++) sums[q][k][i] = 0.0f;
     }
-    for (long long first = range.first; first < range.end; first += teams) {
+    // Everything a row needs is asked for before any of it is used, and with few columns to a thread a turn ahead.
+    constexpr bool kAhead = NV == 1;
+    float up_next[NV][4], mean_next = 0.0f, rstd_next = 0.0f;
+    unsigned code_next[NV];
+    float2 block_next[NV];
+    auto load = [&](long long first) {
         const bool live = first + team < range.end;
-        const long long row = live ? first + team : first;
-        // everything a row needs is asked for before any of it is used
-        float kept[NV][4], up[NV][4], mean = 0.0f, rstd = 0.0f;
-        unsigned code[NV];
-        float2 block[NV];
+        const long long row = live ? first + team : range.first;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
             const bool in = live && col < w;
-            code[k] = in ? *reinterpret_cast<const unsigned*>(p.codes + row * row_bytes + col) : 0u;
-            block[k] = in ? p.blocks[row * row_blocks + col / kCheckpointBlock] : make_float2(0.0f, 0.0f);
-            load_columns<VEC>(p.grad_a + row * p.grad_stride, col, live ? w : 0, up[k]);
+            code_next[k] = in ? *reinterpret_cast<const unsigned*>(p.codes + row * row_bytes + col) : 0u;
+            block_next[k] = in ? p.blocks[row * row_blocks + col / kCheckpointBlock] : make_float2(0.0f, 0.0f);
+            load_columns<VEC>(p.grad_a + row * p.grad_stride, col, live ? w : 0, up_next[k]);
         }
         if (NORM) {
-            mean = p.mean[row];
-            rstd = p.rstd[row];
+            mean_next = p.mean[row];
+            rstd_next = p.rstd[row];
         }
+    };
+    if (kAhead) load(range.first);
+    for (long long first = range.first; first < range.end; first += teams) {
+        const bool live = first + team < range.end;
+        const long long row = first + team;
+        if (!kAhead) load(first);
+        float kept[NV][4], up[NV][4];
+        unsigned code[NV];
+        float2 block[NV];
+        const float mean = mean_next, rstd = rstd_next;
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            code[k] = code_next[k];
+            block[k] = block_next[k];
+#pragma unroll
+            for (int i = 0; i < 4; i++) up[k][i] = up_next[k][i];
+        }
+        if (kAhead && first + teams < range.end) load(first + teams);
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll

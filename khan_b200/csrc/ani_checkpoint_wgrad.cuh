@@ -199,30 +199,37 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                     pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k),
                                       make_float4(sh.dz[g][k][me], sh.dz[g][k + 1][me], sh.dz[g][k + 2][me], sh.dz[g][k + 3][me]));
                 fence_async_smem();
-                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
-                // Columns behind the width: rows of the product that are not stored.
-                float a[kCwK];
-#pragma unroll
-                for (int k = 0; k < kCwK; k += 2) {
-                    const float4 s = *reinterpret_cast<const float4*>(&sh.row[warp][k]);
-                    a[k] = act_value<ACT>(fmaf(fmaf((float)sh.codes[g][k][me], s.x, s.y), gain, bias));
-                    a[k + 1] = act_value<ACT>(fmaf(fmaf((float)sh.codes[g][k + 1][me], s.z, s.w), gain, bias));
-                }
                 // and those of chunk c - 2 this stage of tensor memory
                 if (c >= 2 && !timed_out)
                     timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
                 if (timed_out) sh.failed = 1;
                 __syncwarp();
                 tc_fence_after();
+                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
+                // Columns behind the width: rows of the product that are not stored.
                 const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
 #pragma unroll
                 for (int k0 = 0; k0 < kCwK; k0 += 8) {
-                    float part[8];
+                    // eight at a time, all loads first: one behind the other a value took 100 clocks
+                    float a[8], part[8];
+                    float4 s[4];
+                    unsigned code[8];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k0 + k]);
+                    for (int k = 0; k < 8; k++) code[k] = sh.codes[g][k0 + k][me];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][k0 + 2 * k]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        a[2 * k] = fmaf(fmaf((float)code[2 * k], s[k].x, s[k].y), gain, bias);
+                        a[2 * k + 1] = fmaf(fmaf((float)code[2 * k + 1], s[k].z, s[k].w), gain, bias);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) a[k] = act_value<ACT>(a[k]);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k]);
                     tmem_store8(stage + k0, part);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = a[k0 + k] - part[k];
+                    for (int k = 0; k < 8; k++) part[k] = a[k] - part[k];
                     tmem_store8(stage + kPipeK + k0, part);
                 }
                 tmem_store_wait();
@@ -267,12 +274,13 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
     if (warp == kMlpThreads / 32) tmem_dealloc(tmem, 512);
 }
 
-// The partial products of an element's ranges, added in order: eight threads have a part of the ranges each, four values at
-// a time, and their sums are added in order too.  Zeros for an element without rows.
-constexpr int kCwSumLanes = 32, kCwSumParts = 8;
+// The partial products of an element's ranges, added in order: blockDim.y threads have a part of the ranges each, four values
+// at a time, and their sums are added in order too.  Zeros for an element without rows.
+constexpr int kCwSumLanes = 32, kCwSumParts = 16;
 __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum_kernel(const __grid_constant__ CheckpointWgradParams p)
 {
     __shared__ alignas(16) float part[kCwSumParts][4 * kCwSumLanes];
+    const int parts = blockDim.y;
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.y, first = p.ranges.range_start[t], n = p.ranges.range_start[t + 1] - first;
@@ -280,7 +288,7 @@ __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum
     const int size = p.width * p.out, at = 4 * (blockIdx.x * kCwSumLanes + threadIdx.x);
     const bool vec = size % 4 == 0;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int each = (n + kCwSumParts - 1) / kCwSumParts, begin = threadIdx.y * each, end = min(n, begin + each);
+    const int each = (n + parts - 1) / parts, begin = threadIdx.y * each, end = min(n, begin + each);
 #pragma unroll 4
     for (int k = begin; k < end; k++) {
         float v[4];
@@ -291,11 +299,11 @@ __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum
     }
     store4(&part[threadIdx.y][4 * threadIdx.x], s);
     __syncthreads();
-    const int i = threadIdx.y * kCwSumLanes + threadIdx.x, value = blockIdx.x * 4 * kCwSumLanes + i;
-    if (i < 4 * kCwSumLanes && value < size) {
+    for (int i = threadIdx.y * kCwSumLanes + threadIdx.x; i < 4 * kCwSumLanes; i += parts * kCwSumLanes) {
+        const int value = blockIdx.x * 4 * kCwSumLanes + i;
+        if (value >= size) break;
         float total = part[0][i];
-#pragma unroll
-        for (int k = 1; k < kCwSumParts; k++) total += part[k][i];
+        for (int k = 1; k < parts; k++) total += part[k][i];
         p.grad_w[t][value] = total;
     }
 }

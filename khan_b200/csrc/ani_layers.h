@@ -354,7 +354,12 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     for (int t = 0; t < kTypes; t++) all_written = all_written && (acs_host[t] == 0 ? !p.grad_w[t] : p.ranges.range_start[t + 1] - p.ranges.range_start[t] == 1);
     if (all_written) return ANI_OK;
     const dim3 sum_grid((width * out_width + 4 * kCwSumLanes - 1) / (4 * kCwSumLanes), kTypes);
-    ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, dim3(kCwSumLanes, kCwSumParts), 0, (cudaStream_t)stream, 1, p));
+    // about four ranges to a thread: 58 ranges of 128 x 128 values 7.4 -> 6.4 us with 16 parts instead of 8, 15 of 512 x 512
+    // 15.5 -> 23 us
+    int most = 1, parts = 1;
+    for (int t = 0; t < kTypes; t++) most = std::max(most, p.ranges.range_start[t + 1] - p.ranges.range_start[t]);
+    while (parts < kCwSumParts && 4 * parts < most) parts *= 2;
+    ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, dim3(kCwSumLanes, parts), 0, (cudaStream_t)stream, 1, p));
     return ANI_OK;
 }
 size_t ani_checkpoint_weight_grad_workspace_bytes(int width, int out_width, const int* acs_host)

@@ -212,9 +212,11 @@ __device__ __forceinline__ void zero_sums_without_rows(const ColumnSums<T, Q>& s
                     for (int c = threadIdx.x; c < w; c += kNormThreads) s.out[q][t][c] = T(0);
 }
 
-constexpr int kSumColumns = 32, kSumParts = 8;
+// A thread has a column and every 16th range: the launch is as long as a thread's chain of loads.
+constexpr int kSumColumns = 32, kSumParts = 16;
 template <typename T, int Q>
-__global__ void __launch_bounds__(kSumColumns* kSumParts) column_sums_kernel(const ColumnSums<T, Q> s, const RowRanges r, int w)
+__global__ void __launch_bounds__(kSumColumns* kSumParts)
+    column_sums_kernel(const __grid_constant__ ColumnSums<T, Q> s, const __grid_constant__ RowRanges r, int w)
 {
     __shared__ T part[kSumParts][kSumColumns];
     pdl_wait();
@@ -223,8 +225,10 @@ __global__ void __launch_bounds__(kSumColumns* kSumParts) column_sums_kernel(con
     const int first = r.range_start[t], n = r.range_start[t + 1] - first;
     if (n <= 1 || !s.out[q][t]) return;      // written by the first launch, or not wanted
     T sum = T(0);
-    if (c < w)
+    if (c < w) {
+#pragma unroll 8
         for (int k = threadIdx.y; k < n; k += kSumParts) sum += s.partial[((size_t)(first + k) * Q + q) * w + c];
+    }
     part[threadIdx.y][threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.y == 0 && c < w) {
@@ -322,17 +326,36 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_grad_kernel(const __g
 #pragma unroll
         for (int i = 0; i < 4; i++) dgain[k][i] = dbias[k][i] = T(0);
     }
-    for (long long base = range.first; base < range.end; base += teams) {
+    // with few columns to a thread a row is loaded one turn ahead (at 128 columns a range is four rows to a team)
+    constexpr bool kAhead = NV == 1;
+    T x_next[NV][4], up_next[NV][4], mean_next = T(0), rstd_next = T(0);
+    auto load = [&](long long base) {
         const bool live = base + team < range.end;
-        const long long row = live ? base + team : base;
-        T xhat[NV][4], up[NV][4];
-        const T mean = p.mean[row], rstd = p.rstd[row];
+        const long long row = live ? base + team : range.first;
+        mean_next = p.mean[row];
+        rstd_next = p.rstd[row];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
-            load_columns<VEC>(p.x + row * p.x_stride, col, live ? w : 0, xhat[k]);
-            load_columns<VEC>(p.grad_y + row * p.grad_stride, col, live ? w : 0, up[k]);
+            load_columns<VEC>(p.x + row * p.x_stride, col, live ? w : 0, x_next[k]);
+            load_columns<VEC>(p.grad_y + row * p.grad_stride, col, live ? w : 0, up_next[k]);
         }
+    };
+    if (kAhead) load(range.first);
+    for (long long base = range.first; base < range.end; base += teams) {
+        const bool live = base + team < range.end;
+        const long long row = base + team;
+        if (!kAhead) load(base);
+        T xhat[NV][4], up[NV][4];
+        const T mean = mean_next, rstd = rstd_next;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                xhat[k][i] = x_next[k][i];
+                up[k][i] = up_next[k][i];
+            }
+        if (kAhead && base + teams < range.end) load(base + teams);
         T sum[2] = {T(0), T(0)};
 #pragma unroll
         for (int k = 0; k < NV; k++) {
