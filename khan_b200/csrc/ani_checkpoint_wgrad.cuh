@@ -131,19 +131,28 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
         const int a_bytes = min(kCwTile, row_bytes - m0), b_columns = min(kCwTile, p.out - n0);
         const float2* blocks = p.blocks + range.first * row_blocks + blockIdx.y;
         // the copies of a chunk, by the group; rows of dz behind the range are zeros, bytes there are left as they are
+        constexpr int kAPieces = kCwTile / 16, kBPieces = kCwTile / 4;      // of 16 bytes in a row
+        const int a_row = me / kAPieces, a_at = 16 * (me % kAPieces), b_row = me / kBPieces, b_at = 4 * (me % kBPieces);
         auto fetch = [&](int c) {
             const int k0 = c * kCwK, valid = min(kCwK, n_here - k0);
+            const unsigned char* a_from = a_src + (size_t)(k0 + a_row) * row_bytes + a_at;
 #pragma unroll
-            for (int i = 0; i < kCwK * kCwTile / 16 / 128; i++) {
-                const int row = (i * 128 + me) / (kCwTile / 16), at = 16 * (me % (kCwTile / 16));
-                if (row < valid && at < a_bytes) copy_async<16>(&sh.codes[g][row][at], a_src + (size_t)(k0 + row) * row_bytes + at, 16);
-            }
+            for (int i = 0; i < kCwK * kAPieces / 128; i++)
+                if (a_row + i * (128 / kAPieces) < valid && a_at < a_bytes)
+                    copy_async<16>(&sh.codes[g][a_row + i * (128 / kAPieces)][a_at], a_from + i * (128 / kAPieces) * row_bytes, 16);
             if (p.whole) {
+                const float* b_from = b_src + (size_t)(k0 + b_row) * p.grad_stride + b_at;
+                if (valid == kCwK && b_at < b_columns) {
+                    const long long step = (128 / kBPieces) * p.grad_stride;
 #pragma unroll
-                for (int i = 0; i < kCwK * kCwTile / 4 / 128; i++) {
-                    const int row = (i * 128 + me) / (kCwTile / 4), at = 4 * (me % (kCwTile / 4));
-                    if (at < b_columns)
-                        copy_async<16>(&sh.dz[g][row][at], b_src + (row < valid ? (size_t)(k0 + row) * p.grad_stride + at : 0), row < valid ? 16 : 0);
+                    for (int i = 0; i < kCwK * kBPieces / 128; i++, b_from += step)
+                        copy_async<16>(&sh.dz[g][b_row + i * (128 / kBPieces)][b_at], b_from, 16);
+                } else if (b_at < b_columns) {
+                    for (int i = 0; i < kCwK * kBPieces / 128; i++) {
+                        const int row = b_row + i * (128 / kBPieces);
+                        copy_async<16>(&sh.dz[g][row][b_at], row < valid ? b_from + (size_t)i * (128 / kBPieces) * p.grad_stride : b_src,
+                                       row < valid ? 16 : 0);
+                    }
                 }
             } else if (me < b_columns) {
 #pragma unroll 8

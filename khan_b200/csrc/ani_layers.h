@@ -91,7 +91,8 @@ RowRanges sum_ranges(const int* acs, int width, int sums, size_t size)
     int per_sm = 4;
     if (heavy && quads > 32) per_sm = size > 4 ? (quads > 512 ? 1 : 2) : (quads > 512 ? 2 : 3);
     if (!heavy && quads > 32) per_sm = quads <= 64 ? 3 : quads <= 128 ? 2 : quads <= 256 ? 6 : quads <= 512 ? 4 : 2;
-    return row_ranges(acs, per_sm * kSms, rows, 4 * rows);
+    // up to sixteen rows to a team an element is one range, which saves the second launch (2.1 us of the host, 3 of the device)
+    return row_ranges(acs, per_sm * kSms, rows, *std::max_element(acs, acs + kTypes) <= 16 * rows ? 16 * rows : 4 * rows);
 }
 size_t sums_workspace(const RowRanges& r, int sums, int width, size_t size)
 {
@@ -182,7 +183,7 @@ bool known_activation(int act) { return act >= kActCelu && act <= kActSoftplus; 
 
 // Ranges of the weight gradient: a CTA holds an SM, so the ranges of all tiles are to fill whole waves of SMs.  Of one to
 // four waves the one with the least work in a CTA is taken; setting up a CTA and writing its tile costs about as much as 128
-// rows.
+// rows, and so does the second launch.
 RowRanges wgrad_ranges(const int* acs, int width, int out)
 {
     const long long tiles = (long long)((width + kCwTile - 1) / kCwTile) * ((out + kCwTile - 1) / kCwTile);
@@ -192,7 +193,8 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
         elements += acs[t] > 0;
         most = std::max<long long>(most, acs[t]);
     }
-    long long best = -1, best_rows = (most + kCwK - 1) / kCwK * kCwK;
+    long long best_rows = (most + kCwK - 1) / kCwK * kCwK;      // a range per element
+    long long best = ((elements * tiles + kSms - 1) / kSms) * (best_rows + 128);
     for (int waves = 1; waves <= 4; waves++) {
         const long long budget = (long long)waves * kSms / tiles;      // ranges
         if (budget < elements) continue;
@@ -204,8 +206,8 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
             if (count <= budget) high = mid;
             else low = mid + 1;
         }
-        const long long work = waves * (low * kCwK + 128);
-        if (best < 0 || work < best) {
+        const long long work = waves * (low * kCwK + 128) + (low * kCwK < most ? 128 : 0);
+        if (work < best) {
             best = work;
             best_rows = low * kCwK;
         }

@@ -160,6 +160,62 @@ py::object layer_norm_grad(const at::Tensor& grad, const at::Tensor& x, py::hand
     return py::make_tuple(dx, dgain, dbias);
 }
 
+// A checkpoint: the tensors of its parts, or one buffer that holds them one behind the other (what checkpoint_activation
+// returns: an allocation costs as much host time as half a launch).
+struct Kept {
+    const unsigned char* codes = nullptr;
+    const float *blocks = nullptr, *mean = nullptr, *rstd = nullptr;
+    int64_t n = 0, width = 0;
+    c10::Device device = c10::Device(c10::DeviceType::CPU);
+};
+int64_t kept_bytes(int64_t n, int64_t width, bool norm)
+{
+    return n * (g_layers.row_bytes((int)width) + 8 * g_layers.blocks((int)width) + (norm ? 8 : 0));
+}
+Kept kept_in(const at::Tensor& buffer, int64_t n, int64_t width, bool norm)
+{
+    Kept k;
+    k.n = n;
+    k.width = width;
+    k.device = buffer.device();
+    if (n == 0) return k;
+    k.codes = data<unsigned char>(buffer);
+    k.blocks = reinterpret_cast<const float*>(k.codes + n * g_layers.row_bytes((int)width));
+    if (norm) {
+        k.mean = k.blocks + 2 * n * g_layers.blocks((int)width);
+        k.rstd = k.mean + n;
+    }
+    return k;
+}
+bool read_kept(const at::Tensor& codes, py::handle blocks_or_none, py::handle mean, py::handle rstd, int64_t n, int64_t width,
+               bool norm, Kept* k)
+{
+    k->device = codes.device();
+    if (!k->device.is_cuda() || width < 1 || width > kMaxWidth || !fits(codes, c10::kByte, k->device)) return false;
+    if (blocks_or_none.is_none()) {
+        if (codes.dim() != 1 || codes.numel() != kept_bytes(n, width, norm)) return false;
+        *k = kept_in(codes, n, width, norm);
+        return true;
+    }
+    if (!THPVariable_Check(blocks_or_none.ptr())) return false;
+    const at::Tensor& blocks = THPVariable_Unpack(blocks_or_none.ptr());
+    k->n = n;
+    k->width = width;
+    if (codes.dim() != 2 || codes.size(0) != n || codes.size(1) != g_layers.row_bytes((int)width) || blocks.dim() != 3 ||
+        !fits(blocks, c10::kFloat, k->device) || blocks.size(0) != n || blocks.size(1) != g_layers.blocks((int)width) ||
+        blocks.size(2) != 2 || norm == mean.is_none() || norm == rstd.is_none())
+        return false;
+    k->codes = data<unsigned char>(codes);
+    k->blocks = data<float>(blocks);
+    if (!norm) return true;
+    if (!THPVariable_Check(mean.ptr()) || !THPVariable_Check(rstd.ptr())) return false;
+    const at::Tensor &m = THPVariable_Unpack(mean.ptr()), &s = THPVariable_Unpack(rstd.ptr());
+    if (!fits(m, c10::kFloat, k->device) || m.numel() != n || !fits(s, c10::kFloat, k->device) || s.numel() != n) return false;
+    k->mean = data<float>(m);
+    k->rstd = data<float>(s);
+    return true;
+}
+
 py::object checkpoint_activation(const at::Tensor& z, int act, py::handle gain, py::handle bias, py::handle acs, double eps)
 {
     const auto device = z.device();
@@ -171,50 +227,17 @@ py::object checkpoint_activation(const at::Tensor& z, int act, py::handle gain, 
     if (w < 1 || w > kMaxWidth || !fits_rows(z, c10::kFloat, device, n, w) || !read_rows(acs, n, &r) || norm == bias.is_none() ||
         (norm && (!read_vectors(gain, r, c10::kFloat, device, w, g) || !read_vectors(bias, r, c10::kFloat, device, w, b))))
         return py::none();
-    const int row_bytes = g_layers.row_bytes((int)w), blocks = g_layers.blocks((int)w);
-    if (row_bytes < 0) return py::int_(row_bytes);
     const c10::cuda::CUDAGuard guard(device);
-    at::Tensor a = new_tensor({n, w}, c10::kFloat, device), codes = new_tensor({n, row_bytes}, c10::kByte, device),
-               bl = new_tensor({n, blocks, 2}, c10::kFloat, device), mean, rstd;
-    if (norm) {
-        mean = new_tensor({n}, c10::kFloat, device);
-        rstd = new_tensor({n}, c10::kFloat, device);
-    }
+    at::Tensor a = new_tensor({n, w}, c10::kFloat, device), buffer = new_tensor({kept_bytes(n, w, norm)}, c10::kByte, device);
+    const Kept k = kept_in(buffer, n, w, norm);
     const int rc = g_layers.checkpoint(data<float>(z), row_stride(z), norm ? g : nullptr, norm ? b : nullptr, (int)w, eps, act,
-                                       r.acs, data<float>(a), data<unsigned char>(codes), data<float>(bl),
-                                       norm ? data<float>(mean) : nullptr, norm ? data<float>(rstd) : nullptr, stream_of(device));
+                                       r.acs, data<float>(a), const_cast<unsigned char*>(k.codes), const_cast<float*>(k.blocks),
+                                       const_cast<float*>(k.mean), const_cast<float*>(k.rstd), stream_of(device));
     if (rc) return py::int_(rc);
-    return py::make_tuple(a, codes, bl, norm ? py::cast(mean) : py::none(), norm ? py::cast(rstd) : py::none());
+    return py::make_tuple(a, buffer);
 }
 
-struct Kept {
-    const unsigned char* codes;
-    const float *blocks, *mean = nullptr, *rstd = nullptr;
-    int64_t n, width;
-    c10::Device device = c10::Device(c10::DeviceType::CPU);
-};
-bool read_kept(const at::Tensor& codes, const at::Tensor& blocks, py::handle mean, py::handle rstd, int64_t width, bool norm, Kept* k)
-{
-    k->device = codes.device();
-    if (!k->device.is_cuda() || codes.dim() != 2 || blocks.dim() != 3 || width < 1 || width > kMaxWidth) return false;
-    k->n = codes.size(0);
-    k->width = width;
-    if (!fits(codes, c10::kByte, k->device) || codes.size(1) != g_layers.row_bytes((int)width) ||
-        !fits(blocks, c10::kFloat, k->device) || blocks.size(0) != k->n || blocks.size(1) != g_layers.blocks((int)width) ||
-        blocks.size(2) != 2 || norm == mean.is_none() || norm == rstd.is_none())
-        return false;
-    k->codes = data<unsigned char>(codes);
-    k->blocks = data<float>(blocks);
-    if (!norm) return true;
-    if (!THPVariable_Check(mean.ptr()) || !THPVariable_Check(rstd.ptr())) return false;
-    const at::Tensor &m = THPVariable_Unpack(mean.ptr()), &s = THPVariable_Unpack(rstd.ptr());
-    if (!fits(m, c10::kFloat, k->device) || m.numel() != k->n || !fits(s, c10::kFloat, k->device) || s.numel() != k->n) return false;
-    k->mean = data<float>(m);
-    k->rstd = data<float>(s);
-    return true;
-}
-
-py::object checkpoint_activation_grad(const at::Tensor& codes, const at::Tensor& blocks, py::handle mean, py::handle rstd,
+py::object checkpoint_activation_grad(const at::Tensor& codes, py::handle blocks, py::handle mean, py::handle rstd,
                                       int64_t width, int act, const at::Tensor& grad, py::handle gain, py::handle bias,
                                       py::handle acs)
 {
@@ -222,8 +245,8 @@ py::object checkpoint_activation_grad(const at::Tensor& codes, const at::Tensor&
     Kept k;
     const void *g[4] = {}, *b[4] = {};
     const bool norm = !gain.is_none();
-    if (!read_kept(codes, blocks, mean, rstd, width, norm, &k) || !read_rows(acs, k.n, &r) || norm == bias.is_none() ||
-        !fits_rows(grad, c10::kFloat, k.device, k.n, width) ||
+    if (grad.dim() != 2 || !read_kept(codes, blocks, mean, rstd, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
+        norm == bias.is_none() || !fits_rows(grad, c10::kFloat, k.device, k.n, width) ||
         (norm && (!read_vectors(gain, r, c10::kFloat, k.device, width, g) || !read_vectors(bias, r, c10::kFloat, k.device, width, b))))
         return py::none();
     const c10::cuda::CUDAGuard guard(k.device);
@@ -241,7 +264,7 @@ py::object checkpoint_activation_grad(const at::Tensor& codes, const at::Tensor&
     return py::make_tuple(dz, dsum, norm ? py::cast(dgain) : py::none(), norm ? py::cast(dbias) : py::none());
 }
 
-py::object checkpoint_weight_grad(const at::Tensor& codes, const at::Tensor& blocks, py::handle mean, py::handle rstd,
+py::object checkpoint_weight_grad(const at::Tensor& codes, py::handle blocks, py::handle mean, py::handle rstd,
                                   int64_t width, int act, const at::Tensor& grad, py::handle gain, py::handle bias,
                                   py::handle acs)
 {
@@ -251,8 +274,8 @@ py::object checkpoint_weight_grad(const at::Tensor& codes, const at::Tensor& blo
     const bool norm = !gain.is_none();
     if (grad.dim() != 2 || grad.size(1) < 1 || grad.size(1) > kMaxWidth) return py::none();
     const int64_t out = grad.size(1);
-    if (!read_kept(codes, blocks, mean, rstd, width, norm, &k) || !read_rows(acs, k.n, &r) || norm == bias.is_none() ||
-        !fits_rows(grad, c10::kFloat, k.device, k.n, out) ||
+    if (!read_kept(codes, blocks, mean, rstd, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
+        norm == bias.is_none() || !fits_rows(grad, c10::kFloat, k.device, k.n, out) ||
         (norm && (!read_vectors(gain, r, c10::kFloat, k.device, width, g) || !read_vectors(bias, r, c10::kFloat, k.device, width, b))))
         return py::none();
     const c10::cuda::CUDAGuard guard(k.device);

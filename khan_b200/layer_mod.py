@@ -120,34 +120,58 @@ def layer_norm_grad(grad_y, x, gain, mean, rstd, acs=None):
 class ActivationCheckpoint:
     """What :func:`checkpoint_activation` keeps of the input of an activation: ``codes`` (uint8, a row of
     ``ceil(width / 16) * 16`` bytes per atom), ``blocks`` (float32 ``[n, ceil(width / 128), 2]``: base and step of every 128
-    columns; a code stands for ``base + code * step``), and with a norm ``mean`` and ``rstd`` of the rows."""
+    columns; a code stands for ``base + code * step``), and with a norm ``mean`` and ``rstd`` of the rows.  One made by
+    :func:`checkpoint_activation` has them in one buffer, one made from its parts refers to those."""
 
-    __slots__ = ("codes", "blocks", "width", "activation", "mean", "rstd")
+    __slots__ = ("_parts", "width", "activation", "_rows", "_normed")
 
     def __init__(self, codes, blocks, width: int, activation, mean=None, rstd=None):
-        self.codes, self.blocks, self.width, self.mean, self.rstd = codes, blocks, int(width), mean, rstd
+        self._parts, self.width, self._rows = (codes, blocks, mean, rstd), int(width), codes.shape[0]
+        self._normed = mean is not None
         self.activation = _activation_id(activation)
+
+    @classmethod
+    def _of_buffer(cls, buffer, rows, width, activation, normed):
+        kept = cls.__new__(cls)
+        kept._parts, kept._rows, kept.width, kept.activation, kept._normed = (buffer, None, None, None), rows, width, activation, normed
+        return kept
+
+    def _part(self, which: int):
+        if self._parts[1] is not None:
+            return self._parts[which]
+        n, row, blocks = self._rows, -(-self.width // 16) * 16, -(-self.width // CHECKPOINT_BLOCK)
+        if which >= 2 and not self._normed:
+            return None
+        start = (0, n * row, n * (row + 8 * blocks), n * (row + 8 * blocks + 4))[which]
+        shape = ((n, row), (n, blocks, 2), (n,), (n,))[which]
+        raw = self._parts[0][start:start + int(np.prod(shape, dtype=np.int64)) * (4 if which else 1)]
+        return (raw.view(torch.float32) if which else raw).view(shape)
+
+    codes = property(lambda self: self._part(0))
+    blocks = property(lambda self: self._part(1))
+    mean = property(lambda self: self._part(2))
+    rstd = property(lambda self: self._part(3))
 
     @property
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.blocks, self.mean, self.rstd) if t is not None)
+        return sum(t.numel() * t.element_size() for t in self._parts if t is not None)
 
     def _check(self, where: str, norm: bool):
-        n = self.codes.shape[0]
-        if (self.codes.dtype != torch.uint8 or tuple(self.codes.shape) != (n, -(-self.width // 16) * 16)
-                or self.blocks.dtype != torch.float32
-                or tuple(self.blocks.shape) != (n, -(-self.width // CHECKPOINT_BLOCK), 2)
-                or not self.codes.is_contiguous() or not self.blocks.is_contiguous()):
+        codes, blocks, mean, rstd = (self._part(k) for k in range(4))
+        n = self._rows
+        if (codes.dtype != torch.uint8 or tuple(codes.shape) != (n, -(-self.width // 16) * 16)
+                or blocks.dtype != torch.float32 or tuple(blocks.shape) != (n, -(-self.width // CHECKPOINT_BLOCK), 2)
+                or not codes.is_contiguous() or not blocks.is_contiguous()):
             raise ValueError(f"{where}: not a checkpoint of {n} rows of {self.width} values")
-        if not self.codes.is_cuda:
+        if not codes.is_cuda:
             raise ValueError(f"{where}: the checkpoint must be on a CUDA device (khan_b200 has no CPU path)")
-        if norm != (self.mean is not None) or norm != (self.rstd is not None):
+        if norm != (mean is not None) or norm != (rstd is not None):
             raise ValueError(f"{where}: gain and bias go with the checkpoint of a normalised layer, and only with that")
-        for t in (self.mean, self.rstd) if norm else ():
-            _per_row(t, "mean and rstd", torch.empty((n, 0), dtype=torch.float32, device=self.codes.device))
+        for t in (mean, rstd) if norm else ():
+            _per_row(t, "mean and rstd", torch.empty((n, 0), dtype=torch.float32, device=codes.device))
             if not t.is_contiguous():
                 raise ValueError(f"{where}: mean and rstd must be contiguous")
-        _lib.same_device(self.codes.device, self.blocks, where=where)
+        _lib.same_device(codes.device, blocks, where=where)
 
 
 def _params(gain, bias, acs, x, where: str):
@@ -171,10 +195,8 @@ def checkpoint_activation(z, activation, gain=None, bias=None, acs=None, eps: fl
         acs = _counts(acs, z.shape[0])
         gain, bias = _params(gain, bias, acs, z, "checkpoint_activation")
         out = _lib.torch_ops().checkpoint_activation(z, act, gain, bias, acs, eps)
-    a, codes, blocks, mean, rstd = _done("ani_checkpoint_activation_f32", out)
-    kept = ActivationCheckpoint.__new__(ActivationCheckpoint)
-    kept.codes, kept.blocks, kept.width, kept.activation, kept.mean, kept.rstd = codes, blocks, z.shape[1], act, mean, rstd
-    return a, kept
+    a, buffer = _done("ani_checkpoint_activation_f32", out)
+    return a, ActivationCheckpoint._of_buffer(buffer, *z.shape, act, gain is not None)
 
 
 def _grad_arguments(kept, grad, width, gain, bias, acs, where):
@@ -182,10 +204,10 @@ def _grad_arguments(kept, grad, width, gain, bias, acs, where):
     grad = _rows(grad, "the gradient")
     if grad.dtype != torch.float32:
         raise TypeError(f"{where}: the gradient is {grad.dtype}, expected torch.float32")
-    if grad.shape[0] != kept.codes.shape[0] or (width is not None and grad.shape[1] != width):
+    if grad.shape[0] != kept._rows or (width is not None and grad.shape[1] != width):
         raise ValueError(f"{where}: a gradient {tuple(grad.shape)} does not fit the checkpoint of "
-                         f"{kept.codes.shape[0]} rows of {kept.width} values")
-    _lib.same_device(kept.codes.device, grad, where=where)
+                         f"{kept._rows} rows of {kept.width} values")
+    _lib.same_device(kept._parts[0].device, grad, where=where)
     acs = _counts(acs, grad.shape[0])
     like = torch.empty((0, kept.width), dtype=torch.float32, device=grad.device)
     gain, bias = _params(gain, bias, acs, like, where)
@@ -197,10 +219,10 @@ def checkpoint_activation_grad(kept, grad_a, gain=None, bias=None, acs=None):
     ``grad_sum`` the column sums of ``grad_z`` (the gradient of the bias of the dense layer in front), the last two None
     without a norm."""
     call = _lib.torch_ops().checkpoint_activation_grad
-    out = call(kept.codes, kept.blocks, kept.mean, kept.rstd, kept.width, kept.activation, grad_a, gain, bias, acs)
+    out = call(*kept._parts, kept.width, kept.activation, grad_a, gain, bias, acs)
     if out is None:
         grad_a, gain, bias, acs = _grad_arguments(kept, grad_a, kept.width, gain, bias, acs, "checkpoint_activation_grad")
-        out = call(kept.codes, kept.blocks, kept.mean, kept.rstd, kept.width, kept.activation, grad_a, gain, bias, acs)
+        out = call(*kept._parts, kept.width, kept.activation, grad_a, gain, bias, acs)
     return _done("ani_checkpoint_activation_grad_f32", out)
 
 
@@ -208,10 +230,10 @@ def checkpoint_weight_grad(kept, grad_z, gain=None, bias=None, acs=None):
     """Weight gradient of the dense layer behind a checkpointed activation, ``act(...)^T grad_z`` summed over the rows (of
     each element), ``[width, out]`` or ``[4, width, out]``; the activations are recomputed from the checkpoint."""
     call = _lib.torch_ops().checkpoint_weight_grad
-    out = call(kept.codes, kept.blocks, kept.mean, kept.rstd, kept.width, kept.activation, grad_z, gain, bias, acs)
+    out = call(*kept._parts, kept.width, kept.activation, grad_z, gain, bias, acs)
     if out is None:
         grad_z, gain, bias, acs = _grad_arguments(kept, grad_z, None, gain, bias, acs, "checkpoint_weight_grad")
-        out = call(kept.codes, kept.blocks, kept.mean, kept.rstd, kept.width, kept.activation, grad_z, gain, bias, acs)
+        out = call(*kept._parts, kept.width, kept.activation, grad_z, gain, bias, acs)
     return _done("ani_checkpoint_weight_grad_f32", out)
 
 
