@@ -54,61 +54,76 @@ __device__ __forceinline__ float fast_reciprocal(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Two values at a time: the kernels here are bound by instructions issued, and a packed one does two operations.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fast_exp2(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+__device__ __forceinline__ float2 fast_reciprocal(float2 x) { return make_float2(fast_reciprocal(x.x), fast_reciprocal(x.y)); }
+__device__ __forceinline__ float2 negative_part(float2 x) { return make_float2(min_nan(x.x, 0.0f), min_nan(x.y, 0.0f)); }
+__device__ __forceinline__ float2 positive_part(float2 x) { return make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)); }
+
 // log(1 + e) for e in [0, 1] = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series: what is cut off is below 2e-8 of it.
-__device__ __forceinline__ float log1p_unit(float e)
+__device__ __forceinline__ float2 log1p_unit(float2 e)
 {
-    const float s = e * fast_reciprocal(2.0f + e), t = s * s;
-    float p = 1.0f / 13.0f;
-    p = fmaf(p, t, 1.0f / 11.0f);
-    p = fmaf(p, t, 1.0f / 9.0f);
-    p = fmaf(p, t, 1.0f / 7.0f);
-    p = fmaf(p, t, 0.2f);
-    p = fmaf(p, t, 1.0f / 3.0f);
-    return 2.0f * fmaf(p * t, s, s);
+    const float2 s = __fmul2_rn(e, fast_reciprocal(__fadd2_rn(e, both(2.0f)))), t = __fmul2_rn(s, s);
+    float2 p = both(2.0f / 13.0f);
+    p = __ffma2_rn(p, t, both(2.0f / 11.0f));
+    p = __ffma2_rn(p, t, both(2.0f / 9.0f));
+    p = __ffma2_rn(p, t, both(2.0f / 7.0f));
+    p = __ffma2_rn(p, t, both(2.0f / 5.0f));
+    p = __ffma2_rn(p, t, both(2.0f / 3.0f));
+    p = __ffma2_rn(p, t, both(2.0f));
+    return __fmul2_rn(p, s);
 }
-template <int ACT> __device__ __forceinline__ float act_value(float u)
+template <int ACT> __device__ __forceinline__ float2 act_value(float2 u)
 {
-    if (ACT == kActCelu) return fmaxf(u, 0.0f) + fmaf(0.1f, fast_exp2(min_nan(10.0f * kLog2E * u, 0.0f)), -0.1f);
-    if (ACT == kActGaussian) return fast_exp2(-kLog2E * u * u);
-    if (ACT == kActNormal) return fast_exp2(-0.5f * kLog2E * u * u);
-    return fmaxf(u, 0.0f) + log1p_unit(fast_exp2(-kLog2E * fabsf(u))) - 0.69314718056f;
+    if (ACT == kActCelu) {
+        const float2 e = fast_exp2(negative_part(__fmul2_rn(u, both(10.0f * kLog2E))));
+        return __fadd2_rn(positive_part(u), __ffma2_rn(e, both(0.1f), both(-0.1f)));
+    }
+    if (ACT == kActGaussian) return fast_exp2(__fmul2_rn(__fmul2_rn(u, u), both(-kLog2E)));
+    if (ACT == kActNormal) return fast_exp2(__fmul2_rn(__fmul2_rn(u, u), both(-0.5f * kLog2E)));
+    const float2 l = log1p_unit(fast_exp2(__fmul2_rn(make_float2(fabsf(u.x), fabsf(u.y)), both(-kLog2E))));
+    return __fadd2_rn(__fadd2_rn(positive_part(u), both(-0.69314718056f)), l);
 }
-template <int ACT> __device__ __forceinline__ float act_derivative(float u)
+template <int ACT> __device__ __forceinline__ float2 act_derivative(float2 u)
 {
-    if (ACT == kActCelu) return fast_exp2(min_nan(10.0f * kLog2E * u, 0.0f));
-    if (ACT == kActGaussian) return -2.0f * u * fast_exp2(-kLog2E * u * u);
-    if (ACT == kActNormal) return -u * fast_exp2(-0.5f * kLog2E * u * u);
-    return fast_reciprocal(1.0f + fast_exp2(-kLog2E * u));
+    if (ACT == kActCelu) return fast_exp2(negative_part(__fmul2_rn(u, both(10.0f * kLog2E))));
+    if (ACT == kActGaussian)
+        return __fmul2_rn(__fmul2_rn(u, both(-2.0f)), fast_exp2(__fmul2_rn(__fmul2_rn(u, u), both(-kLog2E))));
+    if (ACT == kActNormal)
+        return __fmul2_rn(make_float2(-u.x, -u.y), fast_exp2(__fmul2_rn(__fmul2_rn(u, u), both(-0.5f * kLog2E))));
+    return fast_reciprocal(__fadd2_rn(fast_exp2(__fmul2_rn(u, both(-kLog2E))), both(1.0f)));
 }
 // All of a thread's values, the choice of the function outside the loop.
-template <int ACT, int NV> __device__ __forceinline__ void act_values_of(float (*u)[4])
+template <int ACT, int NV> __device__ __forceinline__ void act_values_of(float2 (*u)[2])
 {
 #pragma unroll
-    for (int k = 0; k < NV; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[k][i] = act_value<ACT>(u[k][i]);
+    for (int k = 0; k < NV; k++) {
+        u[k][0] = act_value<ACT>(u[k][0]);
+        u[k][1] = act_value<ACT>(u[k][1]);
+    }
 }
-template <int NV> __device__ __forceinline__ void act_values(int act, float (*u)[4])
+template <int NV> __device__ __forceinline__ void act_values(int act, float2 (*u)[2])
 {
     if (act == kActCelu) act_values_of<kActCelu, NV>(u);
     else if (act == kActGaussian) act_values_of<kActGaussian, NV>(u);
     else if (act == kActNormal) act_values_of<kActNormal, NV>(u);
     else act_values_of<kActSoftplus, NV>(u);
 }
-template <int ACT, int NV> __device__ __forceinline__ void act_derivatives_of(float (*u)[4])
+template <int ACT> __device__ __forceinline__ void act_derivatives_of(float2* u)
 {
-#pragma unroll
-    for (int k = 0; k < NV; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[k][i] = act_derivative<ACT>(u[k][i]);
+    u[0] = act_derivative<ACT>(u[0]);
+    u[1] = act_derivative<ACT>(u[1]);
 }
-template <int NV> __device__ __forceinline__ void act_derivatives(int act, float (*u)[4])
+__device__ __forceinline__ void act_derivatives(int act, float2* u)
 {
-    if (act == kActCelu) act_derivatives_of<kActCelu, NV>(u);
-    else if (act == kActGaussian) act_derivatives_of<kActGaussian, NV>(u);
-    else if (act == kActNormal) act_derivatives_of<kActNormal, NV>(u);
-    else act_derivatives_of<kActSoftplus, NV>(u);
+    if (act == kActCelu) act_derivatives_of<kActCelu>(u);
+    else if (act == kActGaussian) act_derivatives_of<kActGaussian>(u);
+    else if (act == kActNormal) act_derivatives_of<kActNormal>(u);
+    else act_derivatives_of<kActSoftplus>(u);
 }
+__device__ __forceinline__ float2 first2(const float* v) { return make_float2(v[0], v[1]); }
+__device__ __forceinline__ float2 last2(const float* v) { return make_float2(v[2], v[3]); }
 
 // Smallest and largest value of a block: over the lanes that share it, NaN if one of them has one.
 template <int TEAM> __device__ __forceinline__ void block_extremes(float* low, float* high)
@@ -163,9 +178,11 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
         float mean = 0.0f, rstd = 1.0f;
         if (NORM) row_statistics<TEAM, NV, VEC>(z, lane, w, p.inv_w, p.eps, scratch, &mean, &rstd);
         const int e = element_of_row(p.groups, row);
+        float2 u[NV][2];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
+            u[k][0] = u[k][1] = both(0.0f);
             float low = __int_as_float(0x7f800000), high = -low;
             if (VEC && col < w) {
                 low = min_nan(min_nan(z[k][0], z[k][1]), min_nan(z[k][2], z[k][3]));
@@ -187,27 +204,33 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
             step = some ? step : 0.0f;
             // rint of 0 .. 255 in one addition: 2^23 + q has its last place at 1, and q in the low bits.  Nothing is above
             // 255: (max - base) (1 / step) is 255 but for four roundings.
+            // (The product by itself: the packed one may be fused with the sum behind it, which rounds once instead of twice.)
+            const float2 d[2] = {__fadd2_rn(first2(z[k]), both(-low)), __fadd2_rn(last2(z[k]), both(-low))};
             unsigned q[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(z[k][i], low), inv), 8388608.0f));
+            for (int i = 0; i < 4; i++)
+                q[i] = __float_as_uint(__fadd_rn(__fmul_rn(i % 2 ? d[i / 2].y : d[i / 2].x, inv), 8388608.0f));
             const unsigned code = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
             *reinterpret_cast<unsigned*>(p.codes + row * row_bytes + col) = code;
             if (col % kCheckpointBlock == 0)
                 p.blocks[row * row_blocks + col / kCheckpointBlock] = make_float2(finite ? low : __int_as_float(0x7fffffff), step);
+            u[k][0] = first2(z[k]);
+            u[k][1] = last2(z[k]);
             if (NORM) {
                 float g[4], h[4];
                 load_columns<VEC>(p.gain[e], col, w, g);
                 load_columns<VEC>(p.bias[e], col, w, h);
-#pragma unroll
-                for (int i = 0; i < 4; i++) z[k][i] = (z[k][i] - mean) * rstd * g[i] + h[i];
+                u[k][0] = __ffma2_rn(__fmul2_rn(__fadd2_rn(u[k][0], both(-mean)), both(rstd)), first2(g), first2(h));
+                u[k][1] = __ffma2_rn(__fmul2_rn(__fadd2_rn(u[k][1], both(-mean)), both(rstd)), last2(g), last2(h));
             }
         }
-        act_values<NV>(p.act, z);
+        act_values<NV>(p.act, u);
         if (!live) continue;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
-            if (col < w) store_columns<VEC>(p.a + row * w, col, w, z[k]);
+            const float a[4] = {u[k][0].x, u[k][0].y, u[k][1].x, u[k][1].y};
+            if (col < w) store_columns<VEC>(p.a + row * w, col, w, a);
         }
         if (NORM && lane == 0) {
             p.mean[row] = mean;
@@ -255,14 +278,11 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
         }
         __syncthreads();
     }
-    float sums[Q][NV][4];
+    float2 sums[Q][NV][2];
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
+    for (int k = 0; k < NV; k++)
 #pragma unroll
-        for (int q = 0; q < Q; q++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sums[q][k][i] = 0.0f;
-    }
+        for (int q = 0; q < Q; q++) sums[q][k][0] = sums[q][k][1] = both(0.0f);
     // Everything a row needs is asked for before any of it is used, and with few columns to a thread a turn ahead.
     constexpr bool kAhead = NV == 1;
     float up_next[NV][4], mean_next = 0.0f, rstd_next = 0.0f;
@@ -289,7 +309,7 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
         const bool live = first + team < range.end;
         const long long row = first + team;
         if (!kAhead) load(first);
-        float kept[NV][4], up[NV][4];
+        float up[NV][4];
         unsigned code[NV];
         float2 block[NV];
         const float mean = mean_next, rstd = rstd_next;
@@ -301,47 +321,57 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
             for (int i = 0; i < 4; i++) up[k][i] = up_next[k][i];
         }
         if (kAhead && first + teams < range.end) load(first + teams);
+        // pairs of columns: what the codes stand for, xhat of that
+        float2 xhat[NV][2], g2[NV][2];
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) kept[k][i] = fmaf((float)((code[k] >> (8 * i)) & 255u), block[k].y, block[k].x);
+            for (int i = 0; i < 2; i++) {
+                const float2 c = make_float2((float)((code[k] >> (16 * i)) & 255u), (float)((code[k] >> (16 * i + 8)) & 255u));
+                xhat[k][i] = __ffma2_rn(c, both(block[k].y), both(block[k].x));
+                g2[k][i] = make_float2(up[k][2 * i], up[k][2 * i + 1]);
+            }
         if constexpr (NORM) {
-            float sum[2] = {0.0f, 0.0f};
+            float2 sum_du = both(0.0f), sum_dx = both(0.0f);
 #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int col = 4 * (lane + k * TEAM);
-                float g[4], h[4], d[1][4];
+                float g[4], h[4];
                 load4(gain_sh + col, g);
                 load4(bias_sh + col, h);
+                // (columns behind the row, and rows behind the range, have a gradient of zero: nothing of them is in a sum)
+                float2 d[2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    kept[k][i] = live && column_in<VEC>(col, i, w) ? (kept[k][i] - mean) * rstd : 0.0f;
-                    d[0][i] = kept[k][i] * g[i] + h[i];
+                for (int i = 0; i < 2; i++) {
+                    xhat[k][i] = __fmul2_rn(__fadd2_rn(xhat[k][i], both(-mean)), both(rstd));
+                    d[i] = __ffma2_rn(xhat[k][i], make_float2(g[2 * i], g[2 * i + 1]), make_float2(h[2 * i], h[2 * i + 1]));
                 }
-                act_derivatives<1>(p.act, d);
+                act_derivatives(p.act, d);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float du = up[k][i] * d[0][i];      // up is zero where there is no value
-                    sums[Q - 2][k][i] += du * kept[k][i];
-                    sums[Q - 1][k][i] += du;
-                    up[k][i] = du * g[i];
-                    sum[0] += up[k][i];
-                    sum[1] += up[k][i] * kept[k][i];
+                for (int i = 0; i < 2; i++) {
+                    const float2 du = __fmul2_rn(g2[k][i], d[i]);
+                    sums[Q - 2][k][i] = __ffma2_rn(du, xhat[k][i], sums[Q - 2][k][i]);
+                    sums[Q - 1][k][i] = __fadd2_rn(sums[Q - 1][k][i], du);
+                    g2[k][i] = __fmul2_rn(du, make_float2(g[2 * i], g[2 * i + 1]));
+                    sum_du = __fadd2_rn(sum_du, g2[k][i]);
+                    sum_dx = __ffma2_rn(g2[k][i], xhat[k][i], sum_dx);
                 }
             }
+            float sum[2] = {sum_du.x + sum_du.y, sum_dx.x + sum_dx.y};
             team_sum<TEAM, 2>(sum, scratch);
-            sum[0] *= p.inv_w;
-            sum[1] *= p.inv_w;
+            const float2 c1 = both(-sum[0] * p.inv_w), c2 = both(-sum[1] * p.inv_w);
 #pragma unroll
             for (int k = 0; k < NV; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) up[k][i] = rstd * (up[k][i] - sum[0] - kept[k][i] * sum[1]);
+                for (int i = 0; i < 2; i++)
+                    g2[k][i] = __fmul2_rn(__ffma2_rn(xhat[k][i], c2, __fadd2_rn(g2[k][i], c1)), both(rstd));
         } else {
-            act_derivatives<NV>(p.act, kept);
 #pragma unroll
-            for (int k = 0; k < NV; k++)
+            for (int k = 0; k < NV; k++) {
+                act_derivatives(p.act, xhat[k]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) up[k][i] *= kept[k][i];
+                for (int i = 0; i < 2; i++) g2[k][i] = __fmul2_rn(g2[k][i], xhat[k][i]);
+            }
         }
         if (!live) continue;
 #pragma unroll
@@ -349,13 +379,20 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
             const int col = 4 * (lane + k * TEAM);
             if (col >= w) break;
 #pragma unroll
-            for (int i = 0; i < 4; i++) sums[0][k][i] += up[k][i];
-            store_columns<VEC>(p.grad_z + row * w, col, w, up[k]);
+            for (int i = 0; i < 2; i++) sums[0][k][i] = __fadd2_rn(sums[0][k][i], g2[k][i]);
+            const float dz[4] = {g2[k][0].x, g2[k][0].y, g2[k][1].x, g2[k][1].y};
+            store_columns<VEC>(p.grad_z + row * w, col, w, dz);
         }
     }
 #pragma unroll
-    for (int q = 0; q < Q; q++)
-        store_column_sums<TEAM, NV>(sums[q], tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, q, w), w);
+    for (int q = 0; q < Q; q++) {
+        float v[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            v[k][0] = sums[q][k][0].x; v[k][1] = sums[q][k][0].y; v[k][2] = sums[q][k][1].x; v[k][3] = sums[q][k][1].y;
+        }
+        store_column_sums<TEAM, NV>(v, tile, column_sums_place(p.sums, p.ranges, range.element, blockIdx.x, q, w), w);
+    }
 }
 
 }  // namespace ani

@@ -21,6 +21,8 @@
 
 namespace ani {
 
+__host__ __device__ __forceinline__ int cw_blocks(int size) { return (size + 31) / 32; }
+
 struct CheckpointWgradParams {
     const unsigned char* codes;
     const float2* blocks;
@@ -30,7 +32,7 @@ struct CheckpointWgradParams {
     const float* grad_z;
     long long grad_stride;
     float* grad_w[kTypes];      // [width][out]
-    float* partial;             // [ranges][width][out]
+    float* partial;             // [ranges][row blocks][column blocks][32 columns][32 rows], blocks of 32 x 32 of the product
     RowRanges ranges;
     int width, out, norm;
     int whole;                  // rows of grad_z are whole 16-byte pieces
@@ -55,7 +57,7 @@ struct CwShared {
     alignas(1024) unsigned char b[kChainGroups][2 * kPipeOperandBytes];
     alignas(16) unsigned char codes[kChainGroups][kCwK][kCwTile];      // a chunk's rows as they are
     alignas(16) float dz[kChainGroups][kCwK][kCwTile];
-    alignas(16) float2 row[kMlpThreads / kWarp][kCwK];      // per warp: step rstd and (base - mean) rstd of the chunk's rows
+    alignas(16) float row[kMlpThreads / kWarp][2 * kCwK];   // per warp and two rows: step rstd of both, (base - mean) rstd of both
     alignas(8) unsigned long long full[kChainGroups], empty[kChainGroups], done[2], drained[2], end;
     unsigned tmem_base;
     int failed;
@@ -196,7 +198,8 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
         for (int r = 0; r < rounds; r++) {
             const int c = r * kCwRound + g;
             if (c < nchunks) {
-                sh.row[warp][lane] = make_float2(block.y * rstd, (block.x - mean) * rstd);
+                sh.row[warp][(lane & ~1) * 2 + (lane & 1)] = block.y * rstd;
+                sh.row[warp][(lane & ~1) * 2 + (lane & 1) + 2] = (block.x - mean) * rstd;
                 copies_wait();
                 group_sync();      // everybody's copies
                 if (c + kChainGroups < nchunks) read_row(c + kChainGroups);
@@ -204,9 +207,15 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                 if (r > 0 && !timed_out) timed_out = !mbar_wait(&sh.empty[g], (unsigned)(r - 1) & 1u);
                 // columns behind the width of dz: columns of the product that are not stored
 #pragma unroll
-                for (int k = 0; k < kCwK; k += 4)
-                    pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k),
-                                      make_float4(sh.dz[g][k][me], sh.dz[g][k + 1][me], sh.dz[g][k + 2][me], sh.dz[g][k + 3][me]));
+                for (int k0 = 0; k0 < kCwK; k0 += 16) {
+                    float v[16];
+#pragma unroll
+                    for (int k = 0; k < 16; k++) v[k] = sh.dz[g][k0 + k][me];
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4)
+                        pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k0 + k),
+                                          make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+                }
                 fence_async_smem();
                 // and those of chunk c - 2 this stage of tensor memory
                 if (c >= 2 && !timed_out)
@@ -220,25 +229,31 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
 #pragma unroll
                 for (int k0 = 0; k0 < kCwK; k0 += 8) {
                     // eight at a time, all loads first: one behind the other a value took 100 clocks
-                    float a[8], part[8];
+                    float2 a[4];
                     float4 s[4];
                     unsigned code[8];
+                    float part[8];
 #pragma unroll
                     for (int k = 0; k < 8; k++) code[k] = sh.codes[g][k0 + k][me];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][k0 + 2 * k]);
+                    for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][2 * k0 + 4 * k]);
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        a[2 * k] = fmaf(fmaf((float)code[2 * k], s[k].x, s[k].y), gain, bias);
-                        a[2 * k + 1] = fmaf(fmaf((float)code[2 * k + 1], s[k].z, s[k].w), gain, bias);
+                        a[k] = __ffma2_rn(make_float2((float)code[2 * k], (float)code[2 * k + 1]), make_float2(s[k].x, s[k].y), make_float2(s[k].z, s[k].w));
+                        a[k] = act_value<ACT>(__ffma2_rn(a[k], both(gain), both(bias)));
                     }
 #pragma unroll
-                    for (int k = 0; k < 8; k++) a[k] = act_value<ACT>(a[k]);
-#pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = tf32_round(a[k]);
+                    for (int k = 0; k < 4; k++) {
+                        part[2 * k] = tf32_round(a[k].x);
+                        part[2 * k + 1] = tf32_round(a[k].y);
+                        a[k] = __fadd2_rn(a[k], make_float2(-part[2 * k], -part[2 * k + 1]));
+                    }
                     tmem_store8(stage + k0, part);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) part[k] = a[k] - part[k];
+                    for (int k = 0; k < 4; k++) {
+                        part[2 * k] = a[k].x;
+                        part[2 * k + 1] = a[k].y;
+                    }
                     tmem_store8(stage + kPipeK + k0, part);
                 }
                 tmem_store_wait();
@@ -261,19 +276,30 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
         tc_fence_after();
         float small[32];
         tmem_load32(lanes + kCwSmall + g * 32, small);
-        producer_sync();      // the operand stages become transposition scratch
+#pragma unroll
+        for (int i = 0; i < 32; i++) sum[i] += small[i];
+        producer_sync();      // the operand stages become transposition scratch; everybody knows of a failure
         if (ok && !sh.failed) {
-            const bool single = p.ranges.range_start[range.element + 1] - p.ranges.range_start[range.element] == 1;
-            float* out = single ? p.grad_w[range.element] : p.partial + (size_t)blockIdx.x * p.width * p.out;
-            float* scratch = reinterpret_cast<float*>(sh.b[0]) + warp * (32 * kMlpScratchStride);
+            const int row_block = m0 / 32 + (warp & 3), column_block = n0 / 32 + g;
+            if (p.ranges.range_start[range.element + 1] - p.ranges.range_start[range.element] != 1) {
+                // as it is held, a column of 32 rows behind the other (rows through the scratch were 2 us)
+                if (row_block < cw_blocks(p.width) && column_block < cw_blocks(p.out)) {
+                    float* to = p.partial + (((size_t)blockIdx.x * cw_blocks(p.width) + row_block) * cw_blocks(p.out) + column_block) * 1024 + lane;
 #pragma unroll
-            for (int i = 0; i < 32; i++) scratch[lane * kMlpScratchStride + i] = sum[i] + small[i];
-            __syncwarp();
-            const int column = n0 + g * 32 + lane, first = m0 + (warp & 3) * 32;
-            if (column < p.out)
+                    for (int i = 0; i < 32; i++) to[32 * i] = sum[i];
+                }
+            } else {
+                float* scratch = reinterpret_cast<float*>(sh.b[0]) + warp * (32 * kMlpScratchStride);
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (first + i < p.width) out[(size_t)(first + i) * p.out + column] = scratch[i * kMlpScratchStride + lane];
+                for (int i = 0; i < 32; i++) scratch[lane * kMlpScratchStride + i] = sum[i];
+                __syncwarp();
+                const int column = column_block * 32 + lane, first = row_block * 32;
+                float* to = p.grad_w[range.element] + (size_t)first * p.out + column;
+                if (column < p.out)
+#pragma unroll 4
+                    for (int i = 0; i < 32; i++, to += p.out)
+                        if (first + i < p.width) *to = scratch[i * kMlpScratchStride + lane];
+            }
         }
     }
     tc_fence_before();
@@ -283,37 +309,38 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
     if (warp == kMlpThreads / 32) tmem_dealloc(tmem, 512);
 }
 
-// The partial products of an element's ranges, added in order: blockDim.y threads have a part of the ranges each, four values
-// at a time, and their sums are added in order too.  Zeros for an element without rows.
-constexpr int kCwSumLanes = 32, kCwSumParts = 16;
+// The partial products of an element's ranges, added in order.  A CTA has half a block, 16 columns of 32 rows; blockDim.y
+// threads have a part of the ranges each, four rows at a time, and their sums are added in order too.  Zeros for an element
+// without rows.
+constexpr int kCwSumLanes = 128, kCwSumParts = 8;
 __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum_kernel(const __grid_constant__ CheckpointWgradParams p)
 {
-    __shared__ alignas(16) float part[kCwSumParts][4 * kCwSumLanes];
-    const int parts = blockDim.y;
+    __shared__ alignas(16) float part[kCwSumParts][16 * 32];
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.y, first = p.ranges.range_start[t], n = p.ranges.range_start[t + 1] - first;
     if (n == 1 || !p.grad_w[t]) return;      // written already, or an element without rows and without a place
-    const int size = p.width * p.out, at = 4 * (blockIdx.x * kCwSumLanes + threadIdx.x);
-    const bool vec = size % 4 == 0;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int parts = blockDim.y, blocks = cw_blocks(p.width) * cw_blocks(p.out), block = blockIdx.x / 2, half = blockIdx.x % 2;
+    const float* from = p.partial + ((size_t)first * blocks + block) * 1024 + half * 512 + 4 * threadIdx.x;
     const int each = (n + parts - 1) / parts, begin = threadIdx.y * each, end = min(n, begin + each);
-#pragma unroll 4
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (int k = begin; k < end; k++) {
         float v[4];
-        if (vec) load_columns<true>(p.partial + (size_t)(first + k) * size, at, size, v);
-        else load_columns<false>(p.partial + (size_t)(first + k) * size, at, size, v);
+        load4(from + (size_t)k * blocks * 1024, v);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[i] += v[i];
     }
     store4(&part[threadIdx.y][4 * threadIdx.x], s);
     __syncthreads();
-    for (int i = threadIdx.y * kCwSumLanes + threadIdx.x; i < 4 * kCwSumLanes; i += parts * kCwSumLanes) {
-        const int value = blockIdx.x * 4 * kCwSumLanes + i;
-        if (value >= size) break;
-        float total = part[0][i];
-        for (int k = 1; k < parts; k++) total += part[k][i];
-        p.grad_w[t][value] = total;
+    // a thread has a place of the half block: 16 columns next to each other in memory
+    const int column0 = block % cw_blocks(p.out) * 32 + half * 16, row0 = block / cw_blocks(p.out) * 32;
+    for (int i = threadIdx.y * kCwSumLanes + threadIdx.x; i < 512; i += parts * kCwSumLanes) {
+        const int c = i % 16, r = i / 16;
+        if (column0 + c >= p.out || row0 + r >= p.width) continue;
+        float total = part[0][c * 32 + r];
+        for (int k = 1; k < parts; k++) total += part[k][c * 32 + r];
+        p.grad_w[t][(size_t)(row0 + r) * p.out + column0 + c] = total;
     }
 }
 

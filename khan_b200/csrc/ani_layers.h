@@ -182,8 +182,8 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
 bool known_activation(int act) { return act >= kActCelu && act <= kActSoftplus; }
 
 // Ranges of the weight gradient: a CTA holds an SM, so the ranges of all tiles are to fill whole waves of SMs.  Of one to
-// four waves the one with the least work in a CTA is taken; setting up a CTA and writing its tile costs about as much as 128
-// rows, and so does the second launch.
+// four waves the one with the least work in a CTA is taken; setting up a CTA and writing its tile costs about as much as 192
+// rows, the second launch as much as 128.
 RowRanges wgrad_ranges(const int* acs, int width, int out)
 {
     const long long tiles = (long long)((width + kCwTile - 1) / kCwTile) * ((out + kCwTile - 1) / kCwTile);
@@ -194,7 +194,7 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
         most = std::max<long long>(most, acs[t]);
     }
     long long best_rows = (most + kCwK - 1) / kCwK * kCwK;      // a range per element
-    long long best = ((elements * tiles + kSms - 1) / kSms) * (best_rows + 128);
+    long long best = ((elements * tiles + kSms - 1) / kSms) * (best_rows + 192);
     for (int waves = 1; waves <= 4; waves++) {
         const long long budget = (long long)waves * kSms / tiles;      // ranges
         if (budget < elements) continue;
@@ -206,7 +206,7 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
             if (count <= budget) high = mid;
             else low = mid + 1;
         }
-        const long long work = waves * (low * kCwK + 128) + (low * kCwK < most ? 128 : 0);
+        const long long work = waves * (low * kCwK + 192) + (low * kCwK < most ? 128 : 0);
         if (work < best) {
             best = work;
             best_rows = low * kCwK;
@@ -355,12 +355,11 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     bool all_written = true;      // by that launch
     for (int t = 0; t < kTypes; t++) all_written = all_written && (acs_host[t] == 0 ? !p.grad_w[t] : p.ranges.range_start[t + 1] - p.ranges.range_start[t] == 1);
     if (all_written) return ANI_OK;
-    const dim3 sum_grid((width * out_width + 4 * kCwSumLanes - 1) / (4 * kCwSumLanes), kTypes);
-    // about four ranges to a thread: 58 ranges of 128 x 128 values 7.4 -> 6.4 us with 16 parts instead of 8, 15 of 512 x 512
-    // 15.5 -> 23 us
+    // about eight ranges to a thread
     int most = 1, parts = 1;
     for (int t = 0; t < kTypes; t++) most = std::max(most, p.ranges.range_start[t + 1] - p.ranges.range_start[t]);
-    while (parts < kCwSumParts && 4 * parts < most) parts *= 2;
+    while (parts < kCwSumParts && 8 * parts < most) parts *= 2;
+    const dim3 sum_grid(2 * cw_blocks(width) * cw_blocks(out_width), kTypes);
     ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, dim3(kCwSumLanes, parts), 0, (cudaStream_t)stream, 1, p));
     return ANI_OK;
 }
@@ -369,7 +368,7 @@ size_t ani_checkpoint_weight_grad_workspace_bytes(int width, int out_width, cons
     long long n = 0;
     if (check_layer(acs_host, width, &n) || out_width < 1 || out_width > kNormMaxWidth) return 0;
     const RowRanges r = wgrad_ranges(acs_host, width, out_width);
-    return one_range_each(r) ? 0 : (size_t)r.range_start[kTypes] * width * out_width * sizeof(float);
+    return one_range_each(r) ? 0 : (size_t)r.range_start[kTypes] * cw_blocks(width) * cw_blocks(out_width) * 1024 * sizeof(float);
 }
 
 }  // extern "C"

@@ -32,6 +32,7 @@ def test_sizes(handle):
     assert small > 0 and large == 2 * small and small % (3 * 128 * 4) == 0
     assert handle.ani_checkpoint_weight_grad_workspace_bytes(128, 64, one) == 0
     assert handle.ani_checkpoint_weight_grad_workspace_bytes(128, 64, many) % (128 * 64 * 4) == 0
+    assert handle.ani_checkpoint_weight_grad_workspace_bytes(1, 1, many) % (32 * 32 * 4) == 0
     assert handle.ani_layer_sums_workspace_bytes(0, many, 3, 4) == handle.ani_checkpoint_weight_grad_workspace_bytes(1, 5000, many) == 0
 
 
