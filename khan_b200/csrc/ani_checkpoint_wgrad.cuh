@@ -217,45 +217,61 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                                           make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
                 }
                 fence_async_smem();
-                // and those of chunk c - 2 this stage of tensor memory
+                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
+                // Columns behind the width: rows of the product that are not stored.
+                // Half of A is formed before the wait for the stage of tensor memory (all of it would not fit the registers).
+                float2 a[kCwK / 4];
+                auto form = [&](int half) {
+#pragma unroll
+                    for (int k0 = 0; k0 < kCwK / 2; k0 += 8) {
+                        // eight at a time, all loads first: one behind the other a value took 100 clocks.  A byte becomes a float
+                        // by an OR and a subtraction: conversions share the unit of the exponentials.
+                        const int row = half * (kCwK / 2) + k0;
+                        float4 s[4];
+                        unsigned code[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) code[k] = sh.codes[g][row + k][me];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][2 * row + 4 * k]);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            float2 q = __fadd2_rn(make_float2(__uint_as_float(code[2 * k] | 0x4b000000u), __uint_as_float(code[2 * k + 1] | 0x4b000000u)),
+                                                  both(-8388608.0f));
+                            q = __ffma2_rn(q, make_float2(s[k].x, s[k].y), make_float2(s[k].z, s[k].w));
+                            a[k0 / 2 + k] = act_value<ACT>(__ffma2_rn(q, both(gain), both(bias)));
+                        }
+                    }
+                };
+                auto store = [&](unsigned to) {
+#pragma unroll
+                    for (int k0 = 0; k0 < kCwK / 2; k0 += 8) {
+                        float part[8];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            part[2 * k] = tf32_round(a[k0 / 2 + k].x);
+                            part[2 * k + 1] = tf32_round(a[k0 / 2 + k].y);
+                            a[k0 / 2 + k] = __fadd2_rn(a[k0 / 2 + k], make_float2(-part[2 * k], -part[2 * k + 1]));
+                        }
+                        tmem_store8(to + k0, part);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            part[2 * k] = a[k0 / 2 + k].x;
+                            part[2 * k + 1] = a[k0 / 2 + k].y;
+                        }
+                        tmem_store8(to + kPipeK + k0, part);
+                    }
+                };
+                form(0);
+                // the products of chunk c - 2 read this stage of tensor memory
                 if (c >= 2 && !timed_out)
                     timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
                 if (timed_out) sh.failed = 1;
                 __syncwarp();
                 tc_fence_after();
-                // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
-                // Columns behind the width: rows of the product that are not stored.
                 const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
-#pragma unroll
-                for (int k0 = 0; k0 < kCwK; k0 += 8) {
-                    // eight at a time, all loads first: one behind the other a value took 100 clocks
-                    float2 a[4];
-                    float4 s[4];
-                    unsigned code[8];
-                    float part[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) code[k] = sh.codes[g][k0 + k][me];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][2 * k0 + 4 * k]);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        a[k] = __ffma2_rn(make_float2((float)code[2 * k], (float)code[2 * k + 1]), make_float2(s[k].x, s[k].y), make_float2(s[k].z, s[k].w));
-                        a[k] = act_value<ACT>(__ffma2_rn(a[k], both(gain), both(bias)));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        part[2 * k] = tf32_round(a[k].x);
-                        part[2 * k + 1] = tf32_round(a[k].y);
-                        a[k] = __fadd2_rn(a[k], make_float2(-part[2 * k], -part[2 * k + 1]));
-                    }
-                    tmem_store8(stage + k0, part);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        part[2 * k] = a[k].x;
-                        part[2 * k + 1] = a[k].y;
-                    }
-                    tmem_store8(stage + kPipeK + k0, part);
-                }
+                store(stage);
+                form(1);
+                store(stage + kCwK / 2);
                 tmem_store_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.full[g]);
@@ -309,19 +325,20 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
     if (warp == kMlpThreads / 32) tmem_dealloc(tmem, 512);
 }
 
-// The partial products of an element's ranges, added in order.  A CTA has half a block, 16 columns of 32 rows; blockDim.y
+// The partial products of an element's ranges, added in order.  A CTA has a quarter of a block, 8 columns of 32 rows; blockDim.y
 // threads have a part of the ranges each, four rows at a time, and their sums are added in order too.  Zeros for an element
 // without rows.
-constexpr int kCwSumLanes = 128, kCwSumParts = 8;
+constexpr int kCwSumColumns = 8, kCwSumLanes = kCwSumColumns * 8, kCwSumParts = 8;
 __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum_kernel(const __grid_constant__ CheckpointWgradParams p)
 {
-    __shared__ alignas(16) float part[kCwSumParts][16 * 32];
+    __shared__ alignas(16) float part[kCwSumParts][kCwSumColumns * 32];
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.y, first = p.ranges.range_start[t], n = p.ranges.range_start[t + 1] - first;
     if (n == 1 || !p.grad_w[t]) return;      // written already, or an element without rows and without a place
-    const int parts = blockDim.y, blocks = cw_blocks(p.width) * cw_blocks(p.out), block = blockIdx.x / 2, half = blockIdx.x % 2;
-    const float* from = p.partial + ((size_t)first * blocks + block) * 1024 + half * 512 + 4 * threadIdx.x;
+    constexpr int pieces = 32 / kCwSumColumns;
+    const int parts = blockDim.y, blocks = cw_blocks(p.width) * cw_blocks(p.out), block = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+    const float* from = p.partial + ((size_t)first * blocks + block) * 1024 + piece * (kCwSumColumns * 32) + 4 * threadIdx.x;
     const int each = (n + parts - 1) / parts, begin = threadIdx.y * each, end = min(n, begin + each);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
@@ -333,10 +350,10 @@ __global__ void __launch_bounds__(kCwSumLanes* kCwSumParts) checkpoint_wgrad_sum
     }
     store4(&part[threadIdx.y][4 * threadIdx.x], s);
     __syncthreads();
-    // a thread has a place of the half block: 16 columns next to each other in memory
-    const int column0 = block % cw_blocks(p.out) * 32 + half * 16, row0 = block / cw_blocks(p.out) * 32;
-    for (int i = threadIdx.y * kCwSumLanes + threadIdx.x; i < 512; i += parts * kCwSumLanes) {
-        const int c = i % 16, r = i / 16;
+    // a thread has a place of the piece: 8 columns next to each other in memory
+    const int column0 = block % cw_blocks(p.out) * 32 + piece * kCwSumColumns, row0 = block / cw_blocks(p.out) * 32;
+    for (int i = threadIdx.y * kCwSumLanes + threadIdx.x; i < kCwSumColumns * 32; i += parts * kCwSumLanes) {
+        const int c = i % kCwSumColumns, r = i / kCwSumColumns;
         if (column0 + c >= p.out || row0 + r >= p.width) continue;
         float total = part[0][c * 32 + r];
         for (int k = 1; k < parts; k++) total += part[k][c * 32 + r];

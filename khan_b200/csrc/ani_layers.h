@@ -182,8 +182,9 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
 bool known_activation(int act) { return act >= kActCelu && act <= kActSoftplus; }
 
 // Ranges of the weight gradient: a CTA holds an SM, so the ranges of all tiles are to fill whole waves of SMs.  Of one to
-// four waves the one with the least work in a CTA is taken; setting up a CTA and writing its tile costs about as much as 192
-// rows, the second launch as much as 128.
+// four waves the one that takes least is chosen, counted in rows of a CTA (33 ns each): setting up a CTA and writing its tile
+// are 192, the second launch 128, and what it reads and writes of partial products 8e-5 a value (37 ranges of 512 x 512 took
+// 25 us more than 9).
 RowRanges wgrad_ranges(const int* acs, int width, int out)
 {
     const long long tiles = (long long)((width + kCwTile - 1) / kCwTile) * ((out + kCwTile - 1) / kCwTile);
@@ -206,7 +207,10 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
             if (count <= budget) high = mid;
             else low = mid + 1;
         }
-        const long long work = waves * (low * kCwK + 192) + (low * kCwK < most ? 128 : 0);
+        long long count = 0;
+        for (int t = 0; t < kTypes; t++) count += (acs[t] + low * kCwK - 1) / (low * kCwK);
+        const long long joined = count > elements ? 128 + count * width * out / 12500 : 0;
+        const long long work = waves * (low * kCwK + 192) + joined;
         if (work < best) {
             best = work;
             best_rows = low * kCwK;
@@ -359,7 +363,7 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     int most = 1, parts = 1;
     for (int t = 0; t < kTypes; t++) most = std::max(most, p.ranges.range_start[t + 1] - p.ranges.range_start[t]);
     while (parts < kCwSumParts && 8 * parts < most) parts *= 2;
-    const dim3 sum_grid(2 * cw_blocks(width) * cw_blocks(out_width), kTypes);
+    const dim3 sum_grid(32 / kCwSumColumns * cw_blocks(width) * cw_blocks(out_width), kTypes);
     ANI_CUDA(launch_chain(checkpoint_wgrad_sum_kernel, sum_grid, dim3(kCwSumLanes, parts), 0, (cudaStream_t)stream, 1, p));
     return ANI_OK;
 }
