@@ -63,6 +63,7 @@ template <bool HEAVY, typename F> cudaError_t with_team(int width, bool vec, F f
         if (quads <= 256) return ANI_TEAM(128, 2);
     } else {
         if (quads <= 64) return ANI_TEAM(32, 2);
+        if (quads <= 96) return ANI_TEAM(32, 3);      // the 384 features
         if (quads <= 128) return ANI_TEAM(32, 4);
         if (quads <= 256) return ANI_TEAM(256, 1);
     }

@@ -268,22 +268,25 @@ __global__ void __launch_bounds__(kNormThreads) layer_norm_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < NV; k++)
             load_columns<VEC>(p.x + (live ? row : 0) * p.x_stride, 4 * (lane + k * TEAM), live ? p.width : 0, x[k]);
+        // asked for before the sums, whose chain is as long as a load from the second-level cache
+        const int e = element_of_row(p.groups, live ? row : 0);
+        T gain[NV][4], bias[NV][4];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            load_columns<VEC>(p.gain[e], 4 * (lane + k * TEAM), p.width, gain[k]);
+            load_columns<VEC>(p.bias[e], 4 * (lane + k * TEAM), p.width, bias[k]);
+        }
         T mean, rstd;
         row_statistics<TEAM, NV, VEC>(x, lane, p.width, p.inv_w, p.eps, scratch, &mean, &rstd);
         if (!live) continue;      // the teams of a CTA of 256 are one, and live
-        const int e = element_of_row(p.groups, row);
-        const T *gain = p.gain[e], *bias = p.bias[e];
         T* y = p.y + row * p.width;
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
             if (col >= p.width) break;
-            T g[4], h[4];
-            load_columns<VEC>(gain, col, p.width, g);
-            load_columns<VEC>(bias, col, p.width, h);
 #pragma unroll
-            for (int i = 0; i < 4; i++) g[i] = (x[k][i] - mean) * rstd * g[i] + h[i];
-            store_columns<VEC>(y, col, p.width, g);
+            for (int i = 0; i < 4; i++) x[k][i] = (x[k][i] - mean) * rstd * gain[k][i] + bias[k][i];
+            store_columns<VEC>(y, col, p.width, x[k]);
         }
         if (lane == 0) {
             p.mean[row] = mean;
