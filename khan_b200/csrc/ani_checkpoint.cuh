@@ -125,13 +125,14 @@ __device__ __forceinline__ void act_derivatives(int act, float2* u)
 __device__ __forceinline__ float2 first2(const float* v) { return make_float2(v[0], v[1]); }
 __device__ __forceinline__ float2 last2(const float* v) { return make_float2(v[2], v[3]); }
 
-// Smallest and largest value of a block: over the lanes that share it, NaN if one of them has one.
+// Smallest and largest value of a block: over the lanes that share it, NaN if one of them has one.  All lanes of the warp
+// take part (volatile: not to be moved to where the result is used, which is not in all of them).
 template <int TEAM> __device__ __forceinline__ void block_extremes(float* low, float* high)
 {
     if (TEAM >= kWarp) {
         float l, h;
-        asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(l) : "f"(*low));
-        asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(h) : "f"(*high));
+        asm volatile("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(l) : "f"(*low));
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(h) : "f"(*high));
         *low = l;
         *high = h;
     } else {

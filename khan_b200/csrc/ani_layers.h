@@ -89,7 +89,7 @@ RowRanges sum_ranges(const int* acs, int width, int sums, size_t size)
     const int quads = (width + 3) / 4;
     const bool heavy = heavy_sums(sums, size);
     const int rows = heavy ? rows_at_once<true>(width) : rows_at_once<false>(width);
-    int per_sm = 4;
+    int per_sm = heavy ? 3 : 4;
     if (heavy && quads > 32) per_sm = size > 4 ? (quads > 512 ? 1 : 2) : (quads > 512 ? 2 : 3);
     if (!heavy && quads > 32) per_sm = quads <= 64 ? 3 : quads <= 128 ? 2 : quads <= 256 ? 6 : quads <= 512 ? 4 : 2;
     // up to sixteen rows to a team an element is one range, which saves the second launch (2.1 us of the host, 3 of the device)

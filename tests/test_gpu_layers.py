@@ -419,6 +419,65 @@ def test_nothing_behind_the_rows_is_written():
         assert (t[size:] == 77).all()
 
 
+def test_offsets_beyond_31_bits():
+    """More than 2^31 values: the last rows of every output, against a call on those rows alone; the sums over rows, whose
+    other rows are zero but for the last."""
+    n, w, out, tail = 530_000, 4096, 8, 40
+    assert n * w > 2 ** 31
+    small = rng_of("offsets").standard_normal((tail, w)).astype(np.float32)
+    gain, bias = torch.rand(w, device=DEV) + 0.5, torch.rand(w, device=DEV) - 0.5
+    x = torch.zeros((n, w), device=DEV)
+    x[-tail:] = dev(small)
+    y, mean, rstd = layer_mod.layer_norm(x, gain, bias)
+    for got, want in zip((y, mean, rstd), layer_mod.layer_norm(dev(small), gain, bias)):
+        assert torch.equal(got[-tail:], want)
+    up = torch.zeros((n, w), device=DEV)
+    up[-tail:] = dev(small) * 1e-2
+    small_up = up[-tail:].clone()
+    dx, dgain, dbias = layer_mod.layer_norm_grad(up, x, gain, mean, rstd)
+    want = layer_mod.layer_norm_grad(small_up, dev(small), gain, mean[-tail:].clone(), rstd[-tail:].clone())
+    assert torch.equal(dx[-tail:], want[0])
+    # the same forty terms in another order: 40 roundings of their sum of magnitudes
+    terms = small_up.abs().sum(0) * 40 * 6e-8
+    assert ((dbias - want[2]).abs() <= terms).all() and ((dgain - want[1]).abs() <= terms * 8).all()
+    del y, dx
+    a, kept = layer_mod.checkpoint_activation(x, "celu", gain, bias)
+    small_a, small_kept = layer_mod.checkpoint_activation(dev(small), "celu", gain, bias)
+    assert torch.equal(a[-tail:], small_a) and torch.equal(kept.codes[-tail:], small_kept.codes) and torch.equal(kept.blocks[-tail:], small_kept.blocks)
+    del a, x
+    dz, dsum, _, _ = layer_mod.checkpoint_activation_grad(kept, up, gain, bias)
+    small_dz, small_dsum, _, _ = layer_mod.checkpoint_activation_grad(small_kept, small_up, gain, bias)
+    assert torch.equal(dz[-tail:], small_dz) and ((dsum - small_dsum).abs() <= small_dz.abs().sum(0) * 40 * 6e-8).all()
+    dz_out = torch.zeros((n, out), device=DEV)
+    dz_out[-tail:] = small_up[:, :out]
+    dw = layer_mod.checkpoint_weight_grad(kept, dz_out, gain, bias)
+    want = layer_mod.checkpoint_weight_grad(small_kept, small_up[:, :out].contiguous(), gain, bias)
+    # |activations| <= 6: xhat is below 5 and the bias below 1; two products of forty rows, each 2^-21 and 40 roundings off
+    assert ((dw - want).abs() <= 2 * (2.0 ** -21 + 80 * 6e-8) * 10 * small_up[:, :out].abs().sum(0)).all()
+
+
+def test_elements_that_share_their_gain():
+    """The same tensor for all elements: the gradient is the sum over all rows."""
+    torch.manual_seed(5)
+    x = torch.randn((50, 20), dtype=torch.float64, device=DEV, requires_grad=True)
+    g, b = (torch.randn(20, dtype=torch.float64, device=DEV, requires_grad=True) for _ in range(2))
+    up = torch.randn((50, 20), dtype=torch.float64, device=DEV)
+    y = layer_mod.layer_norm_autograd(x, [g] * 4, [b] * 4, np.array([20, 10, 0, 20], np.int32))
+    grouped = torch.autograd.grad(y, (x, g, b), up)
+    alone = torch.autograd.grad(layer_mod.layer_norm_autograd(x, g, b), (x, g, b), up)
+    assert torch.equal(grouped[0], alone[0])
+    for p, q in zip(grouped[1:], alone[1:]):
+        assert torch.allclose(p, q, rtol=0, atol=1e-13 * float(up.abs().sum()))
+
+
+def test_counts_in_other_forms():
+    x, gain, bias, up, acs = make(30, 24, np.float32)
+    want = layer_mod.layer_norm(dev(x), dev(gain), dev(bias), acs)
+    for form in (acs.tolist(), acs.astype(np.int64), torch.from_numpy(acs).to(DEV), tuple(dev(gain)) and acs[::1].copy()):
+        for p, q in zip(want, layer_mod.layer_norm(dev(x), tuple(dev(gain)), dev(bias), form)):
+            assert torch.equal(p, q)
+
+
 # ---------------------------------------------------------------- autograd
 def test_layer_norm_autograd_against_differences():
     torch.manual_seed(3)

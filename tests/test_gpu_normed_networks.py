@@ -232,6 +232,20 @@ def test_files_of_networks_with_and_without_norms_are_told_apart(tmp_path):
         normed.load_numpy(files[1])
 
 
+@pytest.mark.parametrize("normed", [False, True])
+def test_the_energy_server_reads_both_kinds_of_files(normed, tmp_path, monkeypatch):
+    from khan_b200 import energy_server
+    tr = trainer(layers=(128, 128, 64, 1), layer_norm=normed, precision="float64")
+    tr.save_numpy(str(tmp_path / "save_file.npz"))
+    served = []
+    monkeypatch.setattr(energy_server, "serve", lambda evaluator, *a, **k: served.append(evaluator))
+    energy_server.main(["--save-dir", str(tmp_path)])
+    X = data().all_Xs[1]
+    want, got = tr.energy_and_gradient(X), served[0].energy_and_gradient(X)
+    assert served[0].model.layer_norm == normed
+    assert abs(want[0] - got[0]) < 1e-12 * max(1, abs(want[0])) and np.allclose(want[1], got[1], rtol=0, atol=1e-12 * max(1, np.abs(want[1]).max()))
+
+
 def test_training_step_is_reproducible():
     """The same batches, twice from the same weights: the operators' sums have one order.  (Torch's products and scatter sums
     of the energies are as reproducible as torch makes them: one batch of one molecule each.)"""
