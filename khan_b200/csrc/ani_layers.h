@@ -46,8 +46,11 @@ bool one_range_each(const RowRanges& r)
     return true;
 }
 
-// The team and the columns per thread for a row of `width` values.  In the activations' backward pass and in double precision
-// a thread holds more than twice as much per column: HEAVY, more threads to a row.
+// The team and the columns per thread for a row of `width` values.  Sixteen columns to a thread once a row is wider than a warp
+// has at four: the fewer threads a row has, the fewer instructions and meetings it costs (backward pass of the activations,
+// 110,000 rows of 512: 101 us with a warp of 16 columns to a thread, 117 with two of 8, 132 with four of 4; 50,000 rows of 1024:
+// 102 us with 64 threads, 110 with 128, 116 with 256).  In double precision 16 columns are too many registers (HEAVY; gradient
+// at 512 columns: 171 us with 64 threads, 187 with 32).
 template <bool HEAVY, typename F> cudaError_t with_team(int width, bool vec, F f)
 {
 #define ANI_TEAM(TEAM, NV)                                                                                            \
@@ -57,17 +60,17 @@ template <bool HEAVY, typename F> cudaError_t with_team(int width, bool vec, F f
     if (quads <= 8) return ANI_TEAM(8, 1);
     if (quads <= 16) return ANI_TEAM(16, 1);
     if (quads <= 32) return ANI_TEAM(32, 1);
+    if (quads <= 64) return ANI_TEAM(32, 2);
     if constexpr (HEAVY) {
-        if (quads <= 64) return ANI_TEAM(64, 1);
         if (quads <= 128) return ANI_TEAM(64, 2);
         if (quads <= 256) return ANI_TEAM(128, 2);
+        if (quads <= 512) return ANI_TEAM(256, 2);
     } else {
-        if (quads <= 64) return ANI_TEAM(32, 2);
         if (quads <= 96) return ANI_TEAM(32, 3);      // the 384 features
         if (quads <= 128) return ANI_TEAM(32, 4);
-        if (quads <= 256) return ANI_TEAM(256, 1);
+        if (quads <= 256) return ANI_TEAM(64, 4);
+        if (quads <= 512) return ANI_TEAM(128, 4);
     }
-    if (quads <= 512) return ANI_TEAM(256, 2);
     return ANI_TEAM(256, 4);
 #undef ANI_TEAM
 }
@@ -81,17 +84,16 @@ template <bool HEAVY> int rows_at_once(int width)
     return rows;
 }
 
-// Whether the launch with `sums` sums of values of `size` bytes takes the larger teams.
-constexpr bool heavy_sums(int sums, size_t size) { return sums > 2 || size > 4; }
-// Ranges of the launches with sums over rows: as many CTAs as are resident at once (their registers, 40 to 224 a thread).
+// Ranges of the launches with sums over rows: as many CTAs as are resident at once (by their registers, 48 to 254 a thread;
+// one more or less costs 10 to 30 %).
 RowRanges sum_ranges(const int* acs, int width, int sums, size_t size)
 {
     const int quads = (width + 3) / 4;
-    const bool heavy = heavy_sums(sums, size);
+    const bool heavy = size > 4;
     const int rows = heavy ? rows_at_once<true>(width) : rows_at_once<false>(width);
-    int per_sm = heavy ? 3 : 4;
-    if (heavy && quads > 32) per_sm = size > 4 ? (quads > 512 ? 1 : 2) : (quads > 512 ? 2 : 3);
-    if (!heavy && quads > 32) per_sm = quads <= 64 ? 3 : quads <= 128 ? 2 : quads <= 256 ? 6 : quads <= 512 ? 4 : 2;
+    const int per_sm = quads <= 32 ? (heavy || sums > 2 ? 3 : 4)
+                       : quads <= 64 ? (heavy ? 2 : sums > 2 ? 3 : 4)
+                                     : (heavy && quads > 512 ? 1 : 2);
     // up to sixteen rows to a team an element is one range, which saves the second launch (2.1 us of the host, 3 of the device)
     return row_ranges(acs, per_sm * kSms, rows, *std::max_element(acs, acs + kTypes) <= 16 * rows ? 16 * rows : 4 * rows);
 }
@@ -147,8 +149,9 @@ int layer_norm(const T* x, long long x_stride, const T* const* gain, const T* co
     p.x = x; p.x_stride = x_stride; p.y = y; p.mean = mean; p.rstd = rstd;
     p.groups = row_groups(acs);
     p.width = width; p.inv_w = T(1) / T(width); p.eps = T(eps);
-    const int grid = rows_grid(n, rows_at_once<false>(width));
-    ANI_CUDA(with_team<false>(width, vec, [&](auto team, auto nv, auto aligned) {
+    constexpr bool heavy = sizeof(T) > 4;
+    const int grid = rows_grid(n, rows_at_once<heavy>(width));
+    ANI_CUDA(with_team<heavy>(width, vec, [&](auto team, auto nv, auto aligned) {
         return launch_chain(layer_norm_kernel<T, team(), nv(), aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return ANI_OK;
@@ -174,7 +177,7 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
     p.grad_y = grad_y; p.grad_stride = grad_stride; p.x = x; p.x_stride = x_stride; p.mean = mean; p.rstd = rstd;
     p.grad_x = grad_x; p.width = width; p.inv_w = T(1) / T(width);
     const int grid = std::max(1, p.ranges.range_start[kTypes]);
-    ANI_CUDA(with_team<heavy_sums(2, sizeof(T))>(width, vec, [&](auto team, auto nv, auto aligned) {
+    ANI_CUDA(with_team<(sizeof(T) > 4)>(width, vec, [&](auto team, auto nv, auto aligned) {
         return launch_chain(layer_norm_grad_kernel<T, team(), nv(), aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
     return column_sums_launch(p.sums, p.ranges, width, (cudaStream_t)stream);
@@ -317,7 +320,7 @@ int ani_checkpoint_activation_grad_f32(const unsigned char* codes, const float* 
     p.grad_a = grad_a; p.grad_stride = grad_stride; p.grad_z = grad_z;
     p.width = width; p.act = activation; p.inv_w = 1.0f / (float)width;
     const int grid = std::max(1, p.ranges.range_start[kTypes]);
-    ANI_CUDA(with_team<true>(width, vec, [&](auto team, auto nv, auto aligned) {
+    ANI_CUDA(with_team<false>(width, vec, [&](auto team, auto nv, auto aligned) {
         return gain_host ? launch_chain(checkpoint_activation_grad_kernel<team(), nv(), true, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p)
                          : launch_chain(checkpoint_activation_grad_kernel<team(), nv(), false, aligned()>, grid, kNormThreads, 0, (cudaStream_t)stream, 1, p);
     }));
