@@ -13,6 +13,10 @@
 // that is not finite, or that spans more than the largest float, has base NaN: its gradients are NaN and not wrong.
 //
 // One byte a value and 8 bytes a block (6 %) instead of the 8 bytes a value that z and a, or a and its derivative, take.
+//
+// 9.06 bytes a value either way.  110,000 x 512 with a norm: forward 92 us with celu, 100 with softplus (78 us of traffic; bound
+// by instructions, 45 for 32 values, 72 % of the issue slots), backward 90 and 96 us (bound by the latency of its loads: a row's
+// sums, xhat and gradients are 126 registers, which leaves 16 warps an SM).
 #pragma once
 
 #include "ani_mlp.cuh"

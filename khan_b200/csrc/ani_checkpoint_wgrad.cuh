@@ -14,6 +14,11 @@
 // The tensor core cuts a sum off at the accumulator's last place, always towards zero, so a long chain of additions drifts:
 // 1e-6 of the value per 32 additions.  So hi hi goes to two accumulators in turn, 128 rows to each, and while one is filled
 // the other is added to float32 sums; the small products (2^-11 of the large ones) have one accumulator for the whole range.
+// Error against float64 in the 2-norm 3e-7 to 4e-7; with all products in the large accumulators 1.0e-6, and no faster.
+//
+// 512 x 512 of 110,000 rows: 405 us, 142 TFLOP/s of float32 products (three times that in tf32, 52 % of its rate).  A chunk and
+// tile takes 1,960 clocks, of which the tensor core is busy 775; 56 % of the issue slots are used, by four staging warps a
+// scheduler whose chains of shared-memory loads, exponentials and tensor-memory stores the rest waits for.
 #pragma once
 
 #include "ani_checkpoint.cuh"

@@ -23,12 +23,16 @@ MAX_WIDTH = 4096
 CHECKPOINT_BLOCK = 128      # columns that share a base and a step
 
 
+_ACTIVATION_IDS = {**activations.KERNEL_ID, **{name: activations.KERNEL_ID[activations.get_fn_by_name(name)]
+                                               for name in activations.get_all_fn_names()}}
+
+
 def _activation_id(activation) -> int:
-    known = isinstance(activation, str) and activation in activations.get_all_fn_names()
-    fn = activations.get_fn_by_name(activation) if known else activation
-    if fn not in activations.KERNEL_ID:
-        raise ValueError(f"no kernel for the activation {activation!r}: one of {activations.get_all_fn_names()}")
-    return activations.KERNEL_ID[fn]
+    """The kernels' number of an activation function of the networks, or of its name."""
+    try:
+        return _ACTIVATION_IDS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"no kernel for the activation {activation!r}: one of {activations.get_all_fn_names()}") from None
 
 
 def _rows(t, name: str, like=None):
@@ -131,7 +135,7 @@ class ActivationCheckpoint:
         self.activation = _activation_id(activation)
 
     @classmethod
-    def _of_buffer(cls, buffer, rows, width, activation, normed):
+    def _of_buffer(cls, buffer, rows, width, activation, normed):      # activation: its number
         kept = cls.__new__(cls)
         kept._parts, kept._rows, kept.width, kept.activation, kept._normed = (buffer, None, None, None), rows, width, activation, normed
         return kept
