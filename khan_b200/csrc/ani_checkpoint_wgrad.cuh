@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
         const float* b_src = p.grad_z + range.first * p.grad_stride + n0;
         const int a_bytes = min(kCwTile, row_bytes - m0), b_columns = min(kCwTile, p.out - n0);
         const float2* blocks = p.blocks + range.first * row_blocks + blockIdx.y;
+        const int b_shift = 32 - __clz(b_columns - 1);      // 2^b_shift >= b_columns
         // the copies of a chunk, by the group; rows of dz behind the range are zeros, bytes there are left as they are
         constexpr int kAPieces = kCwTile / 16, kBPieces = kCwTile / 4;      // of 16 bytes in a row
         const int a_row = me / kAPieces, a_at = 16 * (me % kAPieces), b_row = me / kBPieces, b_at = 4 * (me % kBPieces);
@@ -161,14 +162,16 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                                        row < valid ? 16 : 0);
                     }
                 }
-            } else if (me < b_columns) {
-#pragma unroll 8
-                for (int row = 0; row < kCwK; row++)
-                    copy_async<4>(&sh.dz[g][row][me], b_src + (row < valid ? (size_t)(k0 + row) * p.grad_stride + me : 0), row < valid ? 4 : 0);
+            } else {
+                // single values; a row of few columns is shared out among fewer threads (by one thread 32 copies take 4,400 clocks)
+                const int column = me & ((1 << b_shift) - 1);
+                if (column < b_columns)
+#pragma unroll 4
+                    for (int row = me >> b_shift; row < kCwK; row += 128 >> b_shift)
+                        copy_async<4>(&sh.dz[g][row][column], b_src + (row < valid ? (size_t)(k0 + row) * p.grad_stride + column : 0), row < valid ? 4 : 0);
             }
         };
         auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory"); };
-        if (g < nchunks) fetch(g);
         const float gain = p.norm && a_in ? p.gain[range.element][m0 + me] : 1.0f;
         const float bias = p.norm && a_in ? p.bias[range.element][m0 + me] : 0.0f;
         bool timed_out = false;
@@ -182,10 +185,12 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
             }
             __syncwarp();
             tc_fence_after();
-            float v[32];
-            tmem_load32(lanes + kCwMain + (r & 1) * 128 + g * 32, v);
+            if (g * 32 < n_columns) {
+                float v[32];
+                tmem_load32(lanes + kCwMain + (r & 1) * 128 + g * 32, v);
 #pragma unroll
-            for (int i = 0; i < 32; i++) sum[i] += v[i];
+                for (int i = 0; i < 32; i++) sum[i] += v[i];
+            }
             tc_fence_before();
             mbar_arrive(&sh.drained[r & 1]);
         };
@@ -199,45 +204,49 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
             mean = live && p.norm ? p.mean[range.first + k] : 0.0f;
             rstd = live && p.norm ? p.rstd[range.first + k] : 1.0f;
         };
-        read_row(g);
-        for (int r = 0; r < rounds; r++) {
+        // Turn -1 asks for the first chunks, turn `rounds` only drains.  Every part stands once.
+#pragma unroll 1
+        for (int r = -1; r <= rounds; r++) {
             const int c = r * kCwRound + g;
-            if (c < nchunks) {
+            const bool staged = r >= 0 && c < nchunks;
+            if (staged) {
                 sh.row[warp][(lane & ~1) * 2 + (lane & 1)] = block.y * rstd;
                 sh.row[warp][(lane & ~1) * 2 + (lane & 1) + 2] = (block.x - mean) * rstd;
                 copies_wait();
                 group_sync();      // everybody's copies
-                if (c + kChainGroups < nchunks) read_row(c + kChainGroups);
                 // the products of the group's chunk before read this stage of shared memory
                 if (r > 0 && !timed_out) timed_out = !mbar_wait(&sh.empty[g], (unsigned)(r - 1) & 1u);
                 // columns behind the width of dz: columns of the product that are not stored
+                if (me < n_columns) {
 #pragma unroll
-                for (int k0 = 0; k0 < kCwK; k0 += 16) {
-                    float v[16];
+                    for (int k0 = 0; k0 < kCwK; k0 += 16) {
+                        float v[16];
 #pragma unroll
-                    for (int k = 0; k < 16; k++) v[k] = sh.dz[g][k0 + k][me];
+                        for (int k = 0; k < 16; k++) v[k] = sh.dz[g][k0 + k][me];
 #pragma unroll
-                    for (int k = 0; k < 16; k += 4)
-                        pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k0 + k),
-                                          make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+                        for (int k = 0; k < 16; k += 4)
+                            pipe_store4<true>(sh.b[g], sh.b[g] + kPipeOperandBytes, pipe_offset(me, k0 + k),
+                                              make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+                    }
                 }
                 fence_async_smem();
                 // rows behind the range: their bytes are old ones, times a step of zero; the zeros of B take them out.
                 // Columns behind the width: rows of the product that are not stored.
                 // Half of A is formed before the wait for the stage of tensor memory (all of it would not fit the registers).
-                float2 a[kCwK / 4];
-                auto form = [&](int half) {
+                const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
+#pragma unroll
+                for (int half = 0; half < kCwK; half += kCwK / 2) {
+                    float2 a[kCwK / 4];
 #pragma unroll
                     for (int k0 = 0; k0 < kCwK / 2; k0 += 8) {
                         // eight at a time, all loads first: one behind the other a value took 100 clocks.  A byte becomes a float
                         // by an OR and a subtraction: conversions share the unit of the exponentials.
-                        const int row = half * (kCwK / 2) + k0;
                         float4 s[4];
                         unsigned code[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) code[k] = sh.codes[g][row + k][me];
+                        for (int k = 0; k < 8; k++) code[k] = sh.codes[g][half + k0 + k][me];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][2 * row + 4 * k]);
+                        for (int k = 0; k < 4; k++) s[k] = *reinterpret_cast<const float4*>(&sh.row[warp][2 * (half + k0) + 4 * k]);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             float2 q = __fadd2_rn(make_float2(__uint_as_float(code[2 * k] | 0x4b000000u), __uint_as_float(code[2 * k + 1] | 0x4b000000u)),
@@ -246,8 +255,13 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                             a[k0 / 2 + k] = act_value<ACT>(__ffma2_rn(q, both(gain), both(bias)));
                         }
                     }
-                };
-                auto store = [&](unsigned to) {
+                    if (half == 0) {      // the products of chunk c - 2 read this stage of tensor memory
+                        if (c >= 2 && !timed_out)
+                            timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
+                        if (timed_out) sh.failed = 1;
+                        __syncwarp();
+                        tc_fence_after();
+                    }
 #pragma unroll
                     for (int k0 = 0; k0 < kCwK / 2; k0 += 8) {
                         float part[8];
@@ -257,37 +271,26 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
                             part[2 * k + 1] = tf32_round(a[k0 / 2 + k].y);
                             a[k0 / 2 + k] = __fadd2_rn(a[k0 / 2 + k], make_float2(-part[2 * k], -part[2 * k + 1]));
                         }
-                        tmem_store8(to + k0, part);
+                        tmem_store8(stage + half + k0, part);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             part[2 * k] = a[k0 / 2 + k].x;
                             part[2 * k + 1] = a[k0 / 2 + k].y;
                         }
-                        tmem_store8(to + kPipeK + k0, part);
+                        tmem_store8(stage + kPipeK + half + k0, part);
                     }
-                };
-                form(0);
-                // the products of chunk c - 2 read this stage of tensor memory
-                if (c >= 2 && !timed_out)
-                    timed_out = !mbar_wait(&sh.empty[(c - 2) % kChainGroups], (unsigned)((c - 2) / kChainGroups) & 1u);
-                if (timed_out) sh.failed = 1;
-                __syncwarp();
-                tc_fence_after();
-                const unsigned stage = lanes + kCwA + (c & 1) * 2 * kPipeK;
-                store(stage);
-                form(1);
-                store(stage + kCwK / 2);
+                }
                 tmem_store_wait();
                 tc_fence_before();
                 mbar_arrive(&sh.full[g]);
-                if (c + kChainGroups < nchunks) {
-                    group_sync();      // the group has read the chunk's rows
-                    fetch(c + kChainGroups);
-                }
+            }
+            if (c + kChainGroups < nchunks) {
+                if (staged) group_sync();      // the group has read the chunk's rows
+                fetch(c + kChainGroups);
+                read_row(c + kChainGroups);
             }
             if (r > 0) drain(r - 1);
         }
-        drain(rounds - 1);
         bool ok = !timed_out;
         if (ok && !mbar_wait(&sh.end, 0u)) {
             ok = false;
