@@ -369,8 +369,8 @@ int ani_scale_by_loss_f32(float* grads, long long n, const float* l2s, int n_mol
  * grad_*_host are HOST arrays of four device pointers, one per element (NULL where the element has no rows; the sums of an
  * element without rows are written as zeros where a pointer is given).  1 <= width <= 4096.  Strides count values, are at
  * least the width and need no alignment; rows that are 16-byte aligned are read faster.  Outputs are contiguous and written,
- * not added to.  Nothing is allocated: the calls with sums over rows take a workspace of the stated size (one per call in
- * flight; its content does not matter; size 0: NULL will do).  All sums are formed in a fixed order, in the type of the rows:
+ * not added to.  Nothing is allocated: the calls with sums over rows take a workspace of the stated size, 16-byte aligned
+ * (one per call in flight; its content does not matter; size 0: NULL will do).  All sums are formed in a fixed order, in the type of the rows:
  * results are bit-reproducible.
  *
  * Layer norm:  y = gain (x - mean) rstd + bias,  rstd = 1 / sqrt(variance + eps)  (variance: divided by the width).

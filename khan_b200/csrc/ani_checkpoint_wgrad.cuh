@@ -16,8 +16,8 @@
 // the other is added to float32 sums; the small products (2^-11 of the large ones) have one accumulator for the whole range.
 // Error against float64 in the 2-norm 3e-7 to 4e-7; with all products in the large accumulators 1.0e-6, and no faster.
 //
-// 512 x 512 of 110,000 rows: 405 us, 142 TFLOP/s of float32 products (three times that in tf32, 52 % of its rate).  A chunk and
-// tile takes 1,960 clocks, of which the tensor core is busy 775; 56 % of the issue slots are used, by four staging warps a
+// 512 x 512 of 110,000 rows: 398 us, 145 TFLOP/s of float32 products (three times that in tf32, 53 % of its rate).  A chunk and
+// tile takes 1,900 clocks, of which the tensor core is busy 775; 56 % of the issue slots are used, by four staging warps a
 // scheduler whose chains of shared-memory loads, exponentials and tensor-memory stores the rest waits for.
 #pragma once
 

@@ -173,6 +173,7 @@ int layer_norm_grad(const T* grad_y, long long grad_stride, const T* x, long lon
     if (int rc = take_pointers(grad_bias, acs, p.sums.out[1])) return rc;
     p.ranges = sum_ranges(acs, width, 2, sizeof(T));
     if (sums_workspace(p.ranges, 2, width, sizeof(T)) && !workspace) return ANI_ERR_NULL_POINTER;
+    if (!aligned16({workspace})) return ANI_ERR_MISALIGNED;
     p.sums.partial = static_cast<T*>(workspace);
     p.grad_y = grad_y; p.grad_stride = grad_stride; p.x = x; p.x_stride = x_stride; p.mean = mean; p.rstd = rstd;
     p.grad_x = grad_x; p.width = width; p.inv_w = T(1) / T(width);
@@ -315,6 +316,7 @@ int ani_checkpoint_activation_grad_f32(const unsigned char* codes, const float* 
     if (!aligned16({codes}) || (reinterpret_cast<uintptr_t>(blocks) & 7)) return ANI_ERR_MISALIGNED;
     p.ranges = sum_ranges(acs_host, width, 3, sizeof(float));
     if (sums_workspace(p.ranges, 3, width, sizeof(float)) && !workspace) return ANI_ERR_NULL_POINTER;
+    if (!aligned16({workspace})) return ANI_ERR_MISALIGNED;
     p.sums.partial = static_cast<float*>(workspace);
     p.codes = codes; p.blocks = reinterpret_cast<const float2*>(blocks); p.mean = mean; p.rstd = rstd;
     p.grad_a = grad_a; p.grad_stride = grad_stride; p.grad_z = grad_z;
@@ -347,6 +349,7 @@ int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* bloc
     if (!aligned16({codes}) || (reinterpret_cast<uintptr_t>(blocks) & 7)) return ANI_ERR_MISALIGNED;
     p.ranges = wgrad_ranges(acs_host, width, out_width);
     if (!one_range_each(p.ranges) && !workspace) return ANI_ERR_NULL_POINTER;
+    if (!aligned16({workspace})) return ANI_ERR_MISALIGNED;
     p.codes = codes; p.blocks = reinterpret_cast<const float2*>(blocks); p.mean = mean; p.rstd = rstd;
     p.grad_z = grad_z; p.grad_stride = grad_stride; p.partial = static_cast<float*>(workspace);
     p.width = width; p.out = out_width; p.norm = gain_host != nullptr;

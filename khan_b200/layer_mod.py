@@ -7,6 +7,9 @@ Rows are atoms.  With ``acs`` (host counts of the four elements, as in :mod:`kha
 dimension.  One launch covers all elements (two where sums over many rows are formed), on torch's current stream.  Results
 are bit-reproducible, nothing is kept from one call for the next, and a call can be captured into a CUDA graph.
 
+The functions are not recorded by autograd, but for :func:`layer_norm_autograd`; networks with checkpoints are differentiated
+by :class:`khan_b200.model.nn.MoleculeNN`.
+
 Rows may be strided (a slice of a wider tensor); other layouts are copied.  Widths go from 1 to 4096.  Layer norm takes
 float32 and float64, checkpoints float32.  There is no CPU path.
 """

@@ -49,8 +49,9 @@ def test_layer_norm_checks_need_no_gpu(handle):
             assert fwd(x, stride, v, v, width, eps, counts, y, y, y, None) == -2
         assert grad(x, 127, x, 128, v, x, x, 128, acs, y, v, v, None, None) == grad(x, 128, x, 127, v, x, x, 128, acs, y, v, v, None, None) == -2
         assert grad(x, 128, x, 128, v, x, x, 128, acs, y, None, v, None, None) == grad(x, 128, x, 128, v, x, x, 128, acs, None, v, v, None, None) == -1
-        # many rows need a workspace
+        # many rows need a workspace, 16-byte aligned
         assert grad(x, 128, x, 128, four(x), x, x, 128, (ctypes.c_int * 4)(100000), y, four(y), four(y), None, None) == -1
+        assert grad(x, 128, x, 128, four(x), x, x, 128, (ctypes.c_int * 4)(100000), y, four(y), four(y), y + 8, None) == -9
 
 
 def test_checkpoint_checks_need_no_gpu(handle):
@@ -77,6 +78,8 @@ def test_checkpoint_checks_need_no_gpu(handle):
     assert wgrad(x, x, None, None, None, None, 64, 0, x, 8, 8, acs, None, None, None) == wgrad(x, x, None, None, v, None, 64, 0, x, 8, 8, acs, v, None, None) == -1
     assert wgrad(x, x + 4, None, None, None, None, 64, 0, x, 8, 8, acs, v, None, None) == -9
     assert wgrad(x, x, None, None, None, None, 64, 0, x, 8, 8, many, v, None, None) == -1
+    assert wgrad(x, x, None, None, None, None, 64, 0, x, 8, 8, many, v, x + 8, None) == -9
+    assert grad(x, x, None, None, x, 64, None, None, 64, 0, many, x, v, None, None, x + 4, None) == -9
 
 
 def test_there_is_no_cpu_path():
