@@ -14,8 +14,8 @@
 //
 // One byte a value and 8 bytes a block (6 %) instead of the 8 bytes a value that z and a, or a and its derivative, take.
 //
-// 9.06 bytes a value either way.  110,000 x 512 with a norm: forward 92 us with celu, 100 with softplus (78 us of traffic; bound
-// by instructions, 45 for 32 values, 72 % of the issue slots), backward 90 and 96 us (bound by the latency of its loads: a row's
+// 9.06 bytes a value either way.  110,000 x 512 with a norm: forward 86 us with celu, 93 with softplus (78 us of traffic; bound
+// by instructions, 40 for 32 values, 70 % of the issue slots), backward 90 and 96 us (bound by the latency of its loads: a row's
 // sums, xhat and gradients are 126 registers, which leaves 16 warps an SM).
 #pragma once
 
@@ -182,43 +182,58 @@ __global__ void __launch_bounds__(kNormThreads) checkpoint_activation_kernel(con
             load_columns<VEC>(p.z + row * p.z_stride, 4 * (lane + k * TEAM), w, z[k]);
         float mean = 0.0f, rstd = 1.0f;
         if (NORM) row_statistics<TEAM, NV, VEC>(z, lane, w, p.inv_w, p.eps, scratch, &mean, &rstd);
+        // The extremes of the thread's blocks; what follows from them (a correctly rounded reciprocal among it) is formed for all
+        // of them at once, block k by the lanes k, k + 4, ..: 93 us at 110,000 x 512, 101 with all lanes forming all of them.
+        float low[NV], high[NV];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int col = 4 * (lane + k * TEAM);
+            low[k] = __int_as_float(0x7f800000);
+            high[k] = -low[k];
+            if (VEC && col < w) {
+                low[k] = min_nan(min_nan(z[k][0], z[k][1]), min_nan(z[k][2], z[k][3]));
+                high[k] = max_nan(max_nan(z[k][0], z[k][1]), max_nan(z[k][2], z[k][3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (col + i < w) {
+                        low[k] = min_nan(low[k], z[k][i]);
+                        high[k] = max_nan(high[k], z[k][i]);
+                    }
+            }
+            block_extremes<TEAM>(&low[k], &high[k]);
+        }
+        const int mine = NV == 1 ? 0 : min(lane_id() & 3, NV - 1);
+        float my_low = low[0], my_high = high[0];
+#pragma unroll
+        for (int k = 1; k < NV; k++) {
+            my_low = mine == k ? low[k] : my_low;
+            my_high = mine == k ? high[k] : my_high;
+        }
+        const float spread = __fsub_rn(my_high, my_low), step = __fmul_rn(spread, 1.0f / 255.0f);
+        const bool finite = spread < __int_as_float(0x7f800000), some = finite && step >= 1e-30f;
+        const float my_inv = some ? __frcp_rn(step) : 0.0f;
+        const int my_col = 4 * (lane % TEAM - lane % (TEAM < kWarp ? TEAM : kWarp) + mine * TEAM);      // the block's first column
+        if (live && my_col < w && (NV == 1 ? lane % (TEAM < kWarp ? TEAM : kWarp) == 0 : lane_id() < NV))
+            p.blocks[row * row_blocks + my_col / kCheckpointBlock] = make_float2(finite ? my_low : __int_as_float(0x7fffffff), some ? step : 0.0f);
         const int e = element_of_row(p.groups, row);
         float2 u[NV][2];
 #pragma unroll
         for (int k = 0; k < NV; k++) {
             const int col = 4 * (lane + k * TEAM);
+            const float inv = NV == 1 ? my_inv : __shfl_sync(kFull, my_inv, k);
             u[k][0] = u[k][1] = both(0.0f);
-            float low = __int_as_float(0x7f800000), high = -low;
-            if (VEC && col < w) {
-                low = min_nan(min_nan(z[k][0], z[k][1]), min_nan(z[k][2], z[k][3]));
-                high = max_nan(max_nan(z[k][0], z[k][1]), max_nan(z[k][2], z[k][3]));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (col + i < w) {
-                        low = min_nan(low, z[k][i]);
-                        high = max_nan(high, z[k][i]);
-                    }
-            }
-            block_extremes<TEAM>(&low, &high);
             if (!live || col >= w) continue;
-            const float spread = __fsub_rn(high, low);
-            float step = __fmul_rn(spread, 1.0f / 255.0f);
-            const bool finite = spread < __int_as_float(0x7f800000), some = finite && step >= 1e-30f;
-            const float inv = some ? __frcp_rn(step) : 0.0f;
-            step = some ? step : 0.0f;
             // rint of 0 .. 255 in one addition: 2^23 + q has its last place at 1, and q in the low bits.  Nothing is above
             // 255: (max - base) (1 / step) is 255 but for four roundings.
             // (The product by itself: the packed one may be fused with the sum behind it, which rounds once instead of twice.)
-            const float2 d[2] = {__fadd2_rn(first2(z[k]), both(-low)), __fadd2_rn(last2(z[k]), both(-low))};
+            const float2 d[2] = {__fadd2_rn(first2(z[k]), both(-low[k])), __fadd2_rn(last2(z[k]), both(-low[k]))};
             unsigned q[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 q[i] = __float_as_uint(__fadd_rn(__fmul_rn(i % 2 ? d[i / 2].y : d[i / 2].x, inv), 8388608.0f));
             const unsigned code = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
             *reinterpret_cast<unsigned*>(p.codes + row * row_bytes + col) = code;
-            if (col % kCheckpointBlock == 0)
-                p.blocks[row * row_blocks + col / kCheckpointBlock] = make_float2(finite ? low : __int_as_float(0x7fffffff), step);
             u[k][0] = first2(z[k]);
             u[k][1] = last2(z[k]);
             if (NORM) {
