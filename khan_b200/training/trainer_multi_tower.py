@@ -12,6 +12,10 @@ flat NCCL all-reduce instead of the reference's concat + reduce_mean on the CPU
 (``trainer_multi_tower.py:137-179``).  ``train()`` keeps the reference's schedule: epochs at a
 fixed batch size until the test error has not improved for ``max_local_epoch_count`` epochs, then
 reload the best weights, halve the learning rate and add 128 to the batch size.
+
+Two options go beyond the reference (``khan_b200.model.nn``): ``layer_norm`` normalises the hidden layers,
+``activation_checkpoints`` keeps their activations in 8 bits between the forward and the backward pass of energy
+training; predictions, forces and force training do not use checkpoints.
 """
 from __future__ import annotations
 

@@ -470,6 +470,19 @@ def test_elements_that_share_their_gain():
         assert torch.allclose(p, q, rtol=0, atol=1e-13 * float(up.abs().sum()))
 
 
+@pytest.mark.parametrize("norm", [False, True])
+def test_a_checkpoint_made_of_its_parts(norm):
+    x, gain, bias, up, acs = make(70, 150, np.float32)
+    g, b = (dev(gain), dev(bias)) if norm else (None, None)
+    _, kept = layer_mod.checkpoint_activation(dev(x), layer_mod.activations.softplus, g, b, acs)
+    parts = layer_mod.ActivationCheckpoint(kept.codes.clone(), kept.blocks.clone(), 150, "softplus", *([kept.mean.clone(), kept.rstd.clone()] if norm else []))
+    assert kept.nbytes == parts.nbytes == 70 * (160 + 2 * 8 + (8 if norm else 0)) and (kept.mean is None) != norm
+    for p, q in zip(layer_mod.checkpoint_activation_grad(kept, dev(up), g, b, acs), layer_mod.checkpoint_activation_grad(parts, dev(up), g, b, acs)):
+        assert p is q is None or torch.equal(p, q)
+    dz = dev(up)[:, :33]
+    assert torch.equal(layer_mod.checkpoint_weight_grad(kept, dz, g, b, acs), layer_mod.checkpoint_weight_grad(parts, dz, g, b, acs))
+
+
 def test_counts_in_other_forms():
     x, gain, bias, up, acs = make(30, 24, np.float32)
     want = layer_mod.layer_norm(dev(x), dev(gain), dev(bias), acs)
