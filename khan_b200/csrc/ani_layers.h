@@ -223,6 +223,7 @@ RowRanges wgrad_ranges(const int* acs, int width, int out)
     }
     return row_ranges(acs, 0x7fffffff, kCwK, std::max<long long>(kCwK, best_rows));
 }
+
 }  // namespace
 
 extern "C" {
