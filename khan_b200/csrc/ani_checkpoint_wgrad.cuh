@@ -101,25 +101,34 @@ __global__ void __launch_bounds__(kMlpAllThreads, 1) checkpoint_wgrad_kernel(con
     const unsigned tmem = sh.tmem_base;
 
     if (warp == kMlpThreads / 32) {
-        // ---- the products: one thread ----
+        // ---- the products: one thread.  An instruction is issued when the tensor core is about to take it, so what this thread
+        // waits for elsewhere (300 clocks a barrier) is lost there: the barriers of the next chunk are looked at in between. ----
         if (lane == 0) {
             bool ok = true;
+            unsigned full_seen = 0, drained_seen = 0;
             const unsigned idesc = instr_desc(kCwTile, n_columns);
             for (int c = 0; c < nchunks && ok; c++) {
                 const int g = c % kChainGroups, r = c / kCwRound;
-                if (c % kCwRound == 0 && r >= 2) ok = mbar_wait(&sh.drained[r & 1], (unsigned)(r / 2 - 1) & 1u);
-                ok = ok && mbar_wait(&sh.full[g], (unsigned)(c / kChainGroups) & 1u);
+                if (c % kCwRound == 0 && r >= 2 && !drained_seen) ok = mbar_wait(&sh.drained[r & 1], (unsigned)(r / 2 - 1) & 1u);
+                if (!full_seen) ok = ok && mbar_wait(&sh.full[g], (unsigned)(c / kChainGroups) & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 const unsigned b_hi = smem_u32(sh.b[g]), b_lo = b_hi + kPipeOperandBytes;
                 const unsigned a_hi = tmem + kCwA + (c & 1) * 2 * kPipeK, a_lo = a_hi + kPipeK;
                 const unsigned acc = tmem + kCwMain + (r & 1) * 128;
+                full_seen = drained_seen = 0;
 #pragma unroll
                 for (int ks = 0; ks < kPipeK / 8; ks++) {
                     const unsigned step = ks * 2 * kMlpLbo, col = ks * 8;
                     mma_tf32_ts(acc, a_hi + col, pipe_desc(b_hi + step), idesc, !(c % kCwRound == 0 && ks == 0));
                     mma_tf32_ts(tmem + kCwSmall, a_hi + col, pipe_desc(b_lo + step), idesc, !(c == 0 && ks == 0));
                     mma_tf32_ts(tmem + kCwSmall, a_lo + col, pipe_desc(b_hi + step), idesc, true);
+                    if (ks == 2 && c + 1 < nchunks) {
+                        const int next = c + 1, next_round = next / kCwRound;
+                        full_seen = mbar_test(&sh.full[next % kChainGroups], (unsigned)(next / kChainGroups) & 1u);
+                        if (next % kCwRound == 0 && next_round >= 2)
+                            drained_seen = mbar_test(&sh.drained[next_round & 1], (unsigned)(next_round / 2 - 1) & 1u);
+                    }
                 }
                 mma_commit(&sh.empty[g]);
                 if (c % kCwRound == kCwRound - 1 || c == nchunks - 1) mma_commit(&sh.done[r & 1]);
