@@ -269,11 +269,13 @@ class _LayerNorm(torch.autograd.Function):
         x, mean, rstd, *params = ctx.saved_tensors
         acs, groups = ctx.acs, ctx.groups
         if torch.is_grad_enabled():
+            # With respect to views of the inputs, one for each place: a tensor that serves several elements, or that x was
+            # made from, gets at each place that place's part alone (autograd adds them up and goes on behind x itself).
             with torch.enable_grad():
+                inputs = [t.view_as(t) for t in (x, *params)]
                 ends = np.cumsum(acs if acs is not None else [x.shape[0]]).tolist()
-                y = torch.cat([dense_layer_norm(x[a:b], params[t], params[groups + t], ctx.eps)
+                y = torch.cat([dense_layer_norm(inputs[0][a:b], inputs[1 + t], inputs[1 + groups + t], ctx.eps)
                                for t, (a, b) in enumerate(zip([0] + ends[:-1], ends))])
-                inputs = [x] + list(params)
                 need = [ctx.needs_input_grad[0]] + list(ctx.needs_input_grad[3:])
                 wanted = [k for k, wants in enumerate(need) if wants]
                 got = torch.autograd.grad(y, [inputs[k] for k in wanted], grad_y, create_graph=True, allow_unused=True)

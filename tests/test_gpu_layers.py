@@ -568,3 +568,18 @@ def test_refusals():
         layer_mod.checkpoint_weight_grad(layer_mod.ActivationCheckpoint(kept.codes.cpu(), kept.blocks.cpu(), 16, "celu"), ud)
     with pytest.raises(ValueError, match="CUDA"):
         layer_mod.checkpoint_activation_grad(kept, ud.cpu())
+
+
+def test_second_derivatives_of_norms_that_share_parameters():
+    from test_layers import check_shared_norms
+    check_shared_norms(DEV)
+
+
+def test_second_derivatives_against_differences_with_a_shared_gain():
+    torch.manual_seed(4)
+    acs = np.array([3, 0, 2, 1], np.int32)
+    x = torch.randn((6, 5), dtype=torch.float64, device=DEV, requires_grad=True)
+    g, b = (torch.randn(5, dtype=torch.float64, device=DEV, requires_grad=True) for _ in range(2))
+    fn = lambda x, g, b: layer_mod.layer_norm_autograd(torch.tanh(layer_mod.layer_norm_autograd(x, g, b, eps=1e-3)), [g] * 4, [b, b, g, b], acs, 1e-3)  # noqa: E731
+    assert torch.autograd.gradcheck(fn, (x, g, b))
+    assert torch.autograd.gradgradcheck(fn, (x, g, b))

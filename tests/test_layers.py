@@ -154,3 +154,75 @@ def test_normed_networks_have_named_gains_and_shifts():
     a = torch.nn.functional.layer_norm(a, (16,), net.anns[0].gains[1], net.anns[0].shifts[1], 1e-5)
     want = (net.activation_fn(a) @ net.anns[0].Ws[2] + net.anns[0].bs[2]).reshape(-1)
     assert torch.allclose(net.atom_energies_sorted(x, [5, 0, 0, 0]), want, atol=1e-5)
+
+
+@pytest.fixture
+def norm_on_the_host(monkeypatch):
+    """layer_norm and layer_norm_grad in torch's operations on the host, so that what autograd makes of them needs no GPU."""
+    def norm(x, gain, bias, acs=None, eps=1e-5):
+        mean = x.detach().mean(1)
+        rstd = ((x.detach() - mean[:, None]).square().mean(1) + eps).rsqrt()
+        gain, bias = ([gain], [bias]) if acs is None else (gain, bias)
+        y = [(x.detach()[r] - mean[r, None]) * rstd[r, None] * gain[t].detach().reshape(-1) + bias[t].detach().reshape(-1)
+             for t, r in enumerate(ref.element_rows([len(x)] if acs is None else acs))]
+        return torch.cat(y), mean, rstd
+
+    def norm_grad(grad_y, x, gain, mean, rstd, acs=None):
+        xhat, dx, sums = (x - mean[:, None]) * rstd[:, None], [], []
+        for g, r in zip([gain] if acs is None else gain, ref.element_rows([len(x)] if acs is None else acs)):
+            up = g.reshape(-1) * grad_y[r]
+            dx.append(rstd[r, None] * (up - up.mean(1, keepdim=True) - xhat[r] * (up * xhat[r]).mean(1, keepdim=True)))
+            sums.append(((grad_y[r] * xhat[r]).sum(0), grad_y[r].sum(0)))
+        dg, db = (torch.stack(s) for s in zip(*sums))
+        return (torch.cat(dx), dg, db) if acs is not None else (torch.cat(dx), dg[0], db[0])
+
+    monkeypatch.setattr(layer_mod, "layer_norm", norm)
+    monkeypatch.setattr(layer_mod, "layer_norm_grad", norm_grad)
+
+
+def shared_norms(device="cpu"):
+    """Layer norms whose parameters and rows are not independent of each other, each as (name, output, inputs)."""
+    gen = torch.Generator().manual_seed(5)
+
+    def new(*shape):
+        return torch.randn(shape, generator=gen, dtype=torch.float64).to(device).requires_grad_(True)
+
+    acs = np.array([3, 0, 2, 4], np.int32)
+    x, g, b, h = new(9, 6), new(6), new(6), new(6)
+    yield "one gain and bias for all elements", layer_mod.layer_norm_autograd(x, [g] * 4, [b] * 4, acs, 1e-3), (x, g, b)
+    yield "gains in pairs", layer_mod.layer_norm_autograd(x, [g, h, h, g], [b, g, b, h], acs, 1e-3), (x, g, b, h)
+    yield "bias = gain", layer_mod.layer_norm_autograd(x, g, g, None, 1e-3), (x, g)
+    first = torch.tanh(layer_mod.layer_norm_autograd(x, g, b, None, 1e-3) * 1.5)
+    yield "one gain in two norms", layer_mod.layer_norm_autograd(first, g, b, None, 1e-3), (x, g, b)
+    yield "rows made of the gain", layer_mod.layer_norm_autograd(x * g, g, b, None, 1e-3), (x, g, b)
+
+
+def check_shared_norms(device):
+    """The first derivatives do not depend on whether a second one may follow, and the second ones are those of the formula."""
+    plain = layer_mod.dense_layer_norm
+    for name, y, inputs in shared_norms(device):
+        up = torch.randn(y.shape, generator=torch.Generator().manual_seed(6), dtype=torch.float64).to(device)
+        once = torch.autograd.grad(y, inputs, up, retain_graph=True)
+        twice = torch.autograd.grad(y, inputs, up, create_graph=True)
+        for p, q in zip(once, twice):
+            # sums of at most 54 terms of size below 40 in double precision, formed in another order
+            assert float((p - q.detach()).abs().max()) < 54 * 40 * 2.0 ** -52, name
+        second = torch.autograd.grad(sum((t * t).sum() for t in twice), inputs, materialize_grads=True)
+        x, g, b, *rest = [t.detach().clone().requires_grad_(True) for t in inputs] + ([] if len(inputs) > 2 else [None])
+        rows = ref.element_rows([3, 0, 2, 4])
+        grouped = lambda gs, bs: torch.cat([plain(x[r], p, q, 1e-3) for r, p, q in zip(rows, gs, bs)])  # noqa: E731
+        want = {"one gain and bias for all elements": lambda: grouped([g] * 4, [b] * 4),
+                "gains in pairs": lambda: grouped([g, rest[0], rest[0], g], [b, g, b, rest[0]]),
+                "bias = gain": lambda: plain(x, g, g, 1e-3),
+                "one gain in two norms": lambda: plain(torch.tanh(plain(x, g, b, 1e-3) * 1.5), g, b, 1e-3),
+                "rows made of the gain": lambda: plain(x * g, g, b, 1e-3)}[name]()
+        leaves = [t for t in (x, g, b, *rest) if t is not None]
+        first = torch.autograd.grad(want, leaves, up, create_graph=True)
+        for p, q in zip(twice, first):
+            assert torch.allclose(p, q, rtol=1e-10, atol=1e-10), name
+        for p, q in zip(second, torch.autograd.grad(sum((t * t).sum() for t in first), leaves, materialize_grads=True)):
+            assert torch.allclose(p, q, rtol=1e-9, atol=1e-9 * float(q.abs().max())), name
+
+
+def test_second_derivatives_of_norms_that_share_parameters(norm_on_the_host):
+    check_shared_norms("cpu")
