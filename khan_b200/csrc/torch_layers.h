@@ -187,11 +187,13 @@ Kept kept_in(const at::Tensor& buffer, int64_t n, int64_t width, bool norm)
     }
     return k;
 }
-bool read_kept(const at::Tensor& codes, py::handle blocks_or_none, py::handle mean, py::handle rstd, int64_t n, int64_t width,
-               bool norm, Kept* k)
+// `rows` and `normed` are the checkpoint's own, n and norm what the call is about: the size of one buffer does not tell them
+// (three normalised rows of 16 columns take as many bytes as four that are not).
+bool read_kept(const at::Tensor& codes, py::handle blocks_or_none, py::handle mean, py::handle rstd, int64_t rows, bool normed,
+               int64_t n, int64_t width, bool norm, Kept* k)
 {
     k->device = codes.device();
-    if (!k->device.is_cuda() || width < 1 || width > kMaxWidth || !fits(codes, c10::kByte, k->device)) return false;
+    if (rows != n || normed != norm || !k->device.is_cuda() || width < 1 || width > kMaxWidth || !fits(codes, c10::kByte, k->device)) return false;
     if (blocks_or_none.is_none()) {
         if (codes.dim() != 1 || codes.numel() != kept_bytes(n, width, norm)) return false;
         *k = kept_in(codes, n, width, norm);
@@ -238,14 +240,14 @@ py::object checkpoint_activation(const at::Tensor& z, int act, py::handle gain, 
 }
 
 py::object checkpoint_activation_grad(const at::Tensor& codes, py::handle blocks, py::handle mean, py::handle rstd,
-                                      int64_t width, int act, const at::Tensor& grad, py::handle gain, py::handle bias,
-                                      py::handle acs)
+                                      int64_t rows, bool normed, int64_t width, int act, const at::Tensor& grad,
+                                      py::handle gain, py::handle bias, py::handle acs)
 {
     Rows r;
     Kept k;
     const void *g[4] = {}, *b[4] = {};
     const bool norm = !gain.is_none();
-    if (grad.dim() != 2 || !read_kept(codes, blocks, mean, rstd, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
+    if (grad.dim() != 2 || !read_kept(codes, blocks, mean, rstd, rows, normed, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
         norm == bias.is_none() || !fits_rows(grad, c10::kFloat, k.device, k.n, width) ||
         (norm && (!read_vectors(gain, r, c10::kFloat, k.device, width, g) || !read_vectors(bias, r, c10::kFloat, k.device, width, b))))
         return py::none();
@@ -265,8 +267,8 @@ py::object checkpoint_activation_grad(const at::Tensor& codes, py::handle blocks
 }
 
 py::object checkpoint_weight_grad(const at::Tensor& codes, py::handle blocks, py::handle mean, py::handle rstd,
-                                  int64_t width, int act, const at::Tensor& grad, py::handle gain, py::handle bias,
-                                  py::handle acs)
+                                  int64_t rows, bool normed, int64_t width, int act, const at::Tensor& grad,
+                                  py::handle gain, py::handle bias, py::handle acs)
 {
     Rows r;
     Kept k;
@@ -274,7 +276,7 @@ py::object checkpoint_weight_grad(const at::Tensor& codes, py::handle blocks, py
     const bool norm = !gain.is_none();
     if (grad.dim() != 2 || grad.size(1) < 1 || grad.size(1) > kMaxWidth) return py::none();
     const int64_t out = grad.size(1);
-    if (!read_kept(codes, blocks, mean, rstd, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
+    if (!read_kept(codes, blocks, mean, rstd, rows, normed, grad.size(0), width, norm, &k) || !read_rows(acs, k.n, &r) ||
         norm == bias.is_none() || !fits_rows(grad, c10::kFloat, k.device, k.n, out) ||
         (norm && (!read_vectors(gain, r, c10::kFloat, k.device, width, g) || !read_vectors(bias, r, c10::kFloat, k.device, width, b))))
         return py::none();

@@ -226,10 +226,10 @@ def checkpoint_activation_grad(kept, grad_a, gain=None, bias=None, acs=None):
     ``grad_sum`` the column sums of ``grad_z`` (the gradient of the bias of the dense layer in front), the last two None
     without a norm."""
     call = _lib.torch_ops().checkpoint_activation_grad
-    out = call(*kept._parts, kept.width, kept.activation, grad_a, gain, bias, acs)
+    out = call(*kept._parts, kept._rows, kept._normed, kept.width, kept.activation, grad_a, gain, bias, acs)
     if out is None:
         grad_a, gain, bias, acs = _grad_arguments(kept, grad_a, kept.width, gain, bias, acs, "checkpoint_activation_grad")
-        out = call(*kept._parts, kept.width, kept.activation, grad_a, gain, bias, acs)
+        out = call(*kept._parts, kept._rows, kept._normed, kept.width, kept.activation, grad_a, gain, bias, acs)
     return _done("ani_checkpoint_activation_grad_f32", out)
 
 
@@ -237,10 +237,10 @@ def checkpoint_weight_grad(kept, grad_z, gain=None, bias=None, acs=None):
     """Weight gradient of the dense layer behind a checkpointed activation, ``act(...)^T grad_z`` summed over the rows (of
     each element), ``[width, out]`` or ``[4, width, out]``; the activations are recomputed from the checkpoint."""
     call = _lib.torch_ops().checkpoint_weight_grad
-    out = call(*kept._parts, kept.width, kept.activation, grad_z, gain, bias, acs)
+    out = call(*kept._parts, kept._rows, kept._normed, kept.width, kept.activation, grad_z, gain, bias, acs)
     if out is None:
         grad_z, gain, bias, acs = _grad_arguments(kept, grad_z, None, gain, bias, acs, "checkpoint_weight_grad")
-        out = call(*kept._parts, kept.width, kept.activation, grad_z, gain, bias, acs)
+        out = call(*kept._parts, kept._rows, kept._normed, kept.width, kept.activation, grad_z, gain, bias, acs)
     return _done("ani_checkpoint_weight_grad_f32", out)
 
 

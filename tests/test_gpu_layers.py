@@ -583,3 +583,22 @@ def test_second_derivatives_against_differences_with_a_shared_gain():
     fn = lambda x, g, b: layer_mod.layer_norm_autograd(torch.tanh(layer_mod.layer_norm_autograd(x, g, b, eps=1e-3)), [g] * 4, [b, b, g, b], acs, 1e-3)  # noqa: E731
     assert torch.autograd.gradcheck(fn, (x, g, b))
     assert torch.autograd.gradgradcheck(fn, (x, g, b))
+
+
+@pytest.mark.parametrize("w,kept_rows,normed,given_rows", [(16, 4, False, 3), (16, 3, True, 4), (7, 40, False, 30), (128, 18, False, 17), (200, 28, True, 29)])
+def test_a_checkpoint_of_other_rows_is_refused(w, kept_rows, normed, given_rows):
+    """As many bytes as one of given_rows rows with a norm where it has none, or without one where it has: told apart by what
+    the checkpoint is, not by its size."""
+    size = lambda n, norm: n * (-(-w // 16) * 16 + 8 * -(-w // 128) + (8 if norm else 0))  # noqa: E731
+    x, gain, bias, up, _ = make(kept_rows, w, np.float32)
+    g = (dev(gain[0]), dev(bias[0]))
+    _, kept = layer_mod.checkpoint_activation(dev(x), "celu", *(g if normed else ()))
+    assert kept.nbytes == size(kept_rows, normed) == size(given_rows, not normed)
+    for params in (g, ()):
+        for rows in (given_rows, kept_rows, kept_rows + 1):
+            if rows == kept_rows and normed == bool(params):
+                continue
+            grad = torch.ones((rows, w), device=DEV)
+            for call in (layer_mod.checkpoint_activation_grad, layer_mod.checkpoint_weight_grad):
+                with pytest.raises(ValueError, match="gain and bias go with" if normed != bool(params) else "does not fit"):
+                    call(kept, grad, *params)
