@@ -292,5 +292,9 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm_autograd(x, gain, bias, acs=None, eps: float = 1e-5):
     """:func:`layer_norm` (``y`` alone) that torch.autograd can differentiate, twice where that is asked for."""
     if acs is not None:
+        gain, bias = tuple(gain), tuple(bias)
+        for v, name in ((gain, "gain"), (bias, "bias")):
+            if len(v) != 4:      # eight in all would do for what follows: the fifth gain would be the first bias
+                raise ValueError(f"{name}: rows grouped by element take a list of four vectors, not of {len(v)}")
         return _LayerNorm.apply(x, _counts(acs, x.shape[0]), eps, *gain, *bias)
     return _LayerNorm.apply(x, None, eps, gain, bias)

@@ -226,3 +226,16 @@ def check_shared_norms(device):
 
 def test_second_derivatives_of_norms_that_share_parameters(norm_on_the_host):
     check_shared_norms("cpu")
+
+
+def test_lists_of_gains_and_biases_are_of_four(norm_on_the_host):
+    """Eight vectors in all are not enough: the fifth gain would serve as the first bias."""
+    x, v, acs = torch.ones((5, 3)), torch.ones(3), np.array([2, 1, 1, 1], np.int32)
+    for gains, biases in ((5, 3), (3, 5), (4, 3), (5, 5), (8, 0), (0, 8)):
+        with pytest.raises(ValueError, match="list of four"):
+            layer_mod.layer_norm_autograd(x, [v] * gains, [v] * biases, acs)
+    for gain, bias in ((v, v), ([v] * 4, v), (v, [v] * 4)):
+        with pytest.raises(ValueError, match="list of four"):
+            layer_mod.layer_norm_autograd(x, gain, bias, acs)
+    for four in ([v] * 4, (v,) * 4, torch.ones(4, 3)):
+        assert layer_mod.layer_norm_autograd(x, four, [v] * 4, acs).shape == layer_mod.layer_norm_autograd(x, [v] * 4, four, acs).shape == (5, 3)
