@@ -274,7 +274,7 @@ class _LayerNorm(torch.autograd.Function):
             with torch.enable_grad():
                 inputs = [t.view_as(t) for t in (x, *params)]
                 ends = np.cumsum(acs if acs is not None else [x.shape[0]]).tolist()
-                y = torch.cat([dense_layer_norm(inputs[0][a:b], inputs[1 + t], inputs[1 + groups + t], ctx.eps)
+                y = torch.cat([dense_layer_norm(inputs[0][a:b], inputs[1 + t].reshape(-1), inputs[1 + groups + t].reshape(-1), ctx.eps)
                                for t, (a, b) in enumerate(zip([0] + ends[:-1], ends))])
                 need = [ctx.needs_input_grad[0]] + list(ctx.needs_input_grad[3:])
                 wanted = [k for k, wants in enumerate(need) if wants]
@@ -286,7 +286,7 @@ class _LayerNorm(torch.autograd.Function):
         gain = list(params[:4]) if acs is not None else params[0]
         dx, dgain, dbias = layer_norm_grad(grad_y, x, gain, mean, rstd, acs)
         per_group = [*dgain, *dbias] if acs is not None else [dgain, dbias]
-        return (dx, None, None, *per_group)
+        return (dx, None, None, *(g.view(p.shape) for g, p in zip(per_group, params)))
 
 
 def layer_norm_autograd(x, gain, bias, acs=None, eps: float = 1e-5):

@@ -239,3 +239,24 @@ def test_lists_of_gains_and_biases_are_of_four(norm_on_the_host):
             layer_mod.layer_norm_autograd(x, gain, bias, acs)
     for four in ([v] * 4, (v,) * 4, torch.ones(4, 3)):
         assert layer_mod.layer_norm_autograd(x, four, [v] * 4, acs).shape == layer_mod.layer_norm_autograd(x, [v] * 4, four, acs).shape == (5, 3)
+
+
+@pytest.mark.parametrize("shape", [(6,), (1, 6), (6, 1), (2, 3)])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_gains_and_biases_of_any_shape_with_a_value_per_column(norm_on_the_host, shape, grouped):
+    """Their gradients have their shape, and the values of the vector's, whether a second derivative follows or not."""
+    gen = torch.Generator().manual_seed(7)
+    x, g, b, up = (torch.randn(s, generator=gen, dtype=torch.float64) for s in ((6, 6), 6, 6, (6, 6)))      # as many rows as columns
+    acs = np.array([2, 0, 3, 1], np.int32) if grouped else None
+    results = []
+    for s in ((6,), shape):
+        p, q = (t.reshape(s).clone().requires_grad_(True) for t in (g, b))
+        leaf = x.clone().requires_grad_(True)
+        y = layer_mod.layer_norm_autograd(leaf, [p] * 4 if grouped else p, [q] * 4 if grouped else q, acs)
+        once = torch.autograd.grad(y, (leaf, p, q), up, retain_graph=True)
+        twice = torch.autograd.grad(y, (leaf, p, q), up, create_graph=True)
+        second = torch.autograd.grad((twice[0] ** 2).sum() + (twice[1] ** 2).sum(), (leaf, p))
+        assert once[1].shape == twice[1].shape == once[2].shape == twice[2].shape == second[1].shape == torch.Size(s)
+        results.append([t.detach().reshape(-1) for t in (*once, *twice, *second)])
+    for got, want in zip(results[1], results[0]):
+        assert torch.equal(got, want)
