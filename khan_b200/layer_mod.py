@@ -296,5 +296,6 @@ def layer_norm_autograd(x, gain, bias, acs=None, eps: float = 1e-5):
         for v, name in ((gain, "gain"), (bias, "bias")):
             if len(v) != 4:      # eight in all would do for what follows: the fifth gain would be the first bias
                 raise ValueError(f"{name}: rows grouped by element take a list of four vectors, not of {len(v)}")
-        return _LayerNorm.apply(x, _counts(acs, x.shape[0]), eps, *gain, *bias)
+        # the counts as they are now: the caller's array may be filled with another batch's before the backward pass
+        return _LayerNorm.apply(x, _counts(acs, x.shape[0]).copy(), eps, *gain, *bias)
     return _LayerNorm.apply(x, None, eps, gain, bias)

@@ -260,3 +260,23 @@ def test_gains_and_biases_of_any_shape_with_a_value_per_column(norm_on_the_host,
         results.append([t.detach().reshape(-1) for t in (*once, *twice, *second)])
     for got, want in zip(results[1], results[0]):
         assert torch.equal(got, want)
+
+
+def test_counts_may_change_behind_the_forward_pass(norm_on_the_host):
+    """A batch's counts are often the place of the next batch's: the backward pass goes by those of its forward pass."""
+    gen = torch.Generator().manual_seed(8)
+    x, up = (torch.randn((9, 4), generator=gen, dtype=torch.float64) for _ in range(2))
+    gains, biases = ([torch.randn(4, generator=gen, dtype=torch.float64).requires_grad_(True) for _ in range(4)] for _ in range(2))
+    results = []
+    for counts in (np.array([3, 1, 4, 1], np.int32), torch.tensor([3, 1, 4, 1], dtype=torch.int32)):
+        for twice in (False, True):
+            for change in (False, True):
+                acs = counts.clone() if isinstance(counts, torch.Tensor) else counts.copy()
+                leaf = x.clone().requires_grad_(True)
+                y = layer_mod.layer_norm_autograd(leaf, gains, biases, acs)
+                if change:
+                    acs[:] = acs[[1, 0, 3, 2]]
+                results.append(torch.autograd.grad(y, (leaf, *gains, *biases), up, create_graph=twice))
+    for got in results[1:]:
+        for p, q in zip(got, results[0]):
+            assert torch.allclose(p, q, rtol=1e-10, atol=1e-10)
