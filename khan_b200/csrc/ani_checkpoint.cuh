@@ -359,13 +359,22 @@ __global__ void __launch_bounds__(kNormThreads, NV == 4 ? 2 : 3) checkpoint_acti
                 float g[4], h[4];
                 load4(gain_sh + col, g);
                 load4(bias_sh + col, h);
-                // (columns behind the row, and rows behind the range, have a gradient of zero: nothing of them is in a sum)
+                // Columns behind the row, and rows behind the range, have a gradient of zero and an xhat of zero: nothing of them
+                // is in a sum.  (With the row's rstd their xhat may be infinite, and zero times that is not zero.)
+                const float scale = live && col < w ? rstd : 0.0f;
                 float2 d[2];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    xhat[k][i] = __fmul2_rn(__fadd2_rn(xhat[k][i], both(-mean)), both(rstd));
-                    d[i] = __ffma2_rn(xhat[k][i], make_float2(g[2 * i], g[2 * i + 1]), make_float2(h[2 * i], h[2 * i + 1]));
+                for (int i = 0; i < 2; i++) xhat[k][i] = __fmul2_rn(__fadd2_rn(xhat[k][i], both(-mean)), both(scale));
+                if (!VEC && col < w && col + 4 > w) {      // one thread's columns of a row (a choice for every value: 16 % at 497 columns)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (col + 2 * i >= w) xhat[k][i].x = 0.0f;
+                        if (col + 2 * i + 1 >= w) xhat[k][i].y = 0.0f;
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    d[i] = __ffma2_rn(xhat[k][i], make_float2(g[2 * i], g[2 * i + 1]), make_float2(h[2 * i], h[2 * i + 1]));
                 act_derivatives(p.act, d);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {

@@ -602,3 +602,41 @@ def test_a_checkpoint_of_other_rows_is_refused(w, kept_rows, normed, given_rows)
             for call in (layer_mod.checkpoint_activation_grad, layer_mod.checkpoint_weight_grad):
                 with pytest.raises(ValueError, match="gain and bias go with" if normed != bool(params) else "does not fit"):
                     call(kept, grad, *params)
+
+
+@pytest.mark.parametrize("act", ["celu", "gaussian"])
+@pytest.mark.parametrize("n,w", [(5, 16), (3, 5), (40, 32), (9, 97), (6, 128), (11, 260), (5, 513), (3, 1024), (2, 2050)])
+def test_columns_and_rows_that_are_not_there_add_nothing(n, w, act):
+    """Rows of one large value, whose mean times 1 / sqrt(eps) is beyond float32: zero minus that mean is not a column's xhat,
+    neither behind the width nor behind the last row.  Every column's own xhat is 0, so all is as for rows of zeros."""
+    x, gain, bias, up, acs = make(n, w, np.float32, "gaps", seed=act)
+    g, b = dev(gain), dev(bias)
+    codes = torch.zeros((n, -(-w // 16) * 16), dtype=torch.uint8, device=DEV)
+    blocks = torch.zeros((n, -(-w // 128), 2), device=DEV)
+    mean, rstd = torch.zeros(n, device=DEV), torch.full((n,), EPS ** -0.5, device=DEV)
+    want = layer_mod.checkpoint_activation_grad(layer_mod.ActivationCheckpoint(codes, blocks, w, act, mean, rstd), dev(up), g, b, acs)
+    assert all(torch.isfinite(t).all() for t in want)
+    value = 2.0 ** 123
+    blocks, mean = blocks.clone(), torch.full((n,), value, device=DEV)
+    blocks[:, :, 0] = value
+    got = layer_mod.checkpoint_activation_grad(layer_mod.ActivationCheckpoint(codes, blocks, w, act, mean, rstd), dev(up), g, b, acs)
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+    # bytes behind the width mean nothing, whatever their step
+    codes, blocks = codes.clone(), blocks.clone()
+    codes[:, w:] = 255
+    blocks[:, :, 0], blocks[:, :, 1], mean = 0.0, 2.0 ** 119, torch.zeros(n, device=DEV)
+    got = layer_mod.checkpoint_activation_grad(layer_mod.ActivationCheckpoint(codes, blocks, w, act, mean, rstd), dev(up), g, b, acs)
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+def test_activation_of_constant_rows_of_a_large_value():
+    """The same from the forward pass on: a constant row is its bias, and its gradient that of a row of zeros."""
+    x, gain, bias, up, acs = make(5, 16, np.float32)
+    results = []
+    for value in (2.0 ** 123, 0.0):
+        a, kept = layer_mod.checkpoint_activation(torch.full((5, 16), value, device=DEV), "softplus", dev(gain), dev(bias), acs, EPS)
+        results.append((a, *layer_mod.checkpoint_activation_grad(kept, dev(up), dev(gain), dev(bias), acs)))
+    for p, q in zip(*results):
+        assert torch.isfinite(q).all() and torch.equal(p, q)
