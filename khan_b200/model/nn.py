@@ -258,8 +258,9 @@ class _CheckpointedStacks(torch.autograd.Function):
                 break
             a, checkpoint = layer_mod.checkpoint_activation(z, act_id, gains, shifts, acs, eps)
             kept.append(checkpoint)
-        ctx.save_for_backward(features, *params)
-        ctx.kept, ctx.ranges, ctx.acs, ctx.layers, ctx.normed = kept, ranges, acs, layers, normed
+        # the checkpoints with the tensors: the backward pass lets go of them, however long the energies are kept
+        ctx.save_for_backward(features, *params, *(c._parts[0] for c in kept))
+        ctx.ranges, ctx.acs, ctx.layers, ctx.normed, ctx.activation = ranges, acs, layers, normed, kept[0].activation
         return z.reshape(-1)
 
     @staticmethod
@@ -277,9 +278,12 @@ class _CheckpointedStacks(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("a pass with activation checkpoints can be differentiated once: its activations are kept in "
                                "8 bits (build the network without activation_checkpoints for higher derivatives)")
-        features, *params = ctx.saved_tensors
+        features, *saved = ctx.saved_tensors
         acs, ranges, layers = ctx.acs, ctx.ranges, ctx.layers
+        params, buffers = saved[:-(layers - 1)], saved[-(layers - 1):]
         per_layer = _CheckpointedStacks._by_layer(params, layers, ctx.normed)
+        kept = [layer_mod.ActivationCheckpoint._of_buffer(b, features.shape[0], layer[0][0].shape[1], ctx.activation, ctx.normed)
+                for b, layer in zip(buffers, per_layer)]
         grads = [None] * layers
         dz = grad_energy.reshape(-1, 1)
         dsum = torch.stack([dz[s:e].sum(0) for s, e in ranges])
@@ -290,7 +294,7 @@ class _CheckpointedStacks(torch.autograd.Function):
                 dws = [features[s:e].t() @ dz[s:e] for s, e in ranges]
             else:
                 gains, shifts = per_layer[k - 1][2:]
-                dws = layer_mod.checkpoint_weight_grad(ctx.kept[k - 1], dz, gains, shifts, acs)
+                dws = layer_mod.checkpoint_weight_grad(kept[k - 1], dz, gains, shifts, acs)
             grads[k] = [*dws, *dsum, *(g for four in norm_grads for g in four)]
             if k == 0:
                 break
@@ -298,7 +302,7 @@ class _CheckpointedStacks(torch.autograd.Function):
             for (s, e), w in zip(ranges, ws):
                 if e > s:
                     torch.mm(dz[s:e], w.t(), out=da[s:e])
-            dz, dsum, *norm_grads = layer_mod.checkpoint_activation_grad(ctx.kept[k - 1], da, gains, shifts, acs)
+            dz, dsum, *norm_grads = layer_mod.checkpoint_activation_grad(kept[k - 1], da, gains, shifts, acs)
             norm_grads = norm_grads if ctx.normed else ()
         return (None,) * 6 + tuple(g for layer in grads for g in layer)
 

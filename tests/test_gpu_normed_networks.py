@@ -296,3 +296,54 @@ def test_training_step_is_reproducible():
     for other in grads[1:]:
         for p, q in zip(grads[0], other):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("normed", [False, True])
+def test_the_backward_pass_lets_go_of_the_checkpoints(normed, monkeypatch):
+    """As of every tensor that autograd keeps: gone when the graph has been used, though the energies are still there; kept
+    with retain_graph; and not to be written to in between."""
+    import torch
+    from khan_b200 import layer_mod
+    acs = np.array([4000, 3000, 900, 600], np.int32)
+    net = network(layer_norm=normed, activation_checkpoints=True)
+    features, up = rows(acs)
+    sizes, keep, last = [], layer_mod.checkpoint_activation, []
+
+    def watched(*args, **kw):
+        a, kept = keep(*args, **kw)
+        sizes.append(kept.nbytes)
+        last[:] = [kept] if watch else []
+        return a, kept
+
+    monkeypatch.setattr(layer_mod, "checkpoint_activation", watched)
+    watch = False
+
+    def held(retain):
+        for p in net.get_parameters():
+            p.grad = None
+        sizes.clear()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        energy = net.atom_energies_sorted(features, acs)
+        forward = torch.cuda.memory_allocated() - before
+        grads = torch.autograd.grad((energy * up).sum(), net.get_parameters(), retain_graph=retain)
+        assert len(grads) == len(net.get_parameters())
+        del grads
+        torch.cuda.synchronize()
+        return energy, forward, torch.cuda.memory_allocated() - before
+
+    held(False)      # the libraries' workspaces
+    energy, forward, after = held(False)
+    assert len(sizes) == 3 and forward >= sum(sizes) > 2_000_000
+    assert after < 500_000      # the energies, 34 kB, and what the allocator rounds up
+    with pytest.raises(RuntimeError, match="second time"):
+        energy.sum().backward()
+    del energy
+    energy, _, after = held(True)
+    assert after >= sum(sizes)
+    del energy
+    watch = True
+    energy = net.atom_energies_sorted(features, acs)
+    last[0].codes.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        energy.sum().backward()
