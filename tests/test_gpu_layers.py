@@ -640,3 +640,41 @@ def test_activation_of_constant_rows_of_a_large_value():
         results.append((a, *layer_mod.checkpoint_activation_grad(kept, dev(up), dev(gain), dev(bias), acs)))
     for p, q in zip(*results):
         assert torch.isfinite(q).all() and torch.equal(p, q)
+
+
+# rows, width, out, norm, activation: ranges of a few hundred rows; widths whose rows are copied value by value; one column;
+# so many tiles that an element of 5,000 rows is one range, with one accumulator for all of its small products
+EXACT = [(20000, 256, 192, True, "celu"), (20000, 256, 192, False, "softplus"), (20000, 256, 97, True, "softplus"), (13750, 64, 1, False, "celu"),
+         (13750, 128, 128, True, "gaussian"), (20000, 1700, 1700, True, "celu"), (20000, 1700, 1601, False, "softplus")]
+
+
+@pytest.mark.parametrize("n,w,out,norm,act", EXACT)
+def test_weight_gradient_over_long_sums(n, w, out, norm, act):
+    """Relative error in the 2-norm, below 7e-7.  What is expected of it:
+      the tensor core cuts a sum off at its last place, by half a place in the mean: 2^-24 / m of a sum with mantissa m, 4.3e-8
+      over the mantissas.  A chain of 128 rows is 16 such sums; the i-th is i / 16 of the last, seen along it (terms of either
+      sign): 8.5 * 4.3e-8 = 3.7e-7, always towards zero.  (A chain over a range of 544 rows: 1.5e-6; over 5,000: 1.4e-5.)
+      The small products have one chain for a range, but are 2^-11 of the sum: 5,000 rows 1e-8.
+      What the parts leave out, low times low and the low parts' own last places: 1e-7.
+      Activations: an exponential of 2^-22, a reciprocal and up to ten roundings, 2e-7 of their root mean square at most.
+    Together (square root of the sum of squares) 4.3e-7."""
+    x, gain, bias, _, acs = make(n, w, np.float32, seed=out)
+    dz = dev((rng_of("long", n, w, out).standard_normal((n, out)) * 1e-2).astype(np.float32))
+    g, b = (dev(gain), dev(bias)) if norm else (None, None)
+    _, kept = layer_mod.checkpoint_activation(dev(x), act, g, b, acs)
+    dw = layer_mod.checkpoint_weight_grad(kept, dz, g, b, acs).double()
+    blocks = kept.blocks.double()[:, torch.arange(w) // 128]
+    z = blocks[:, :, 0] + kept.codes[:, :w].double() * blocks[:, :, 1]
+    for t, rows in enumerate(ref.element_rows(acs)):
+        u = z[rows]
+        if norm:
+            u = (u - kept.mean.double()[rows, None]) * kept.rstd.double()[rows, None] * g[t].double() + b[t].double()
+        if act == "celu":
+            a = torch.where(u >= 0, u, 0.1 * torch.expm1(10 * u.clamp(max=0)))
+        elif act == "gaussian":
+            a = torch.exp(-u * u)
+        else:
+            a = u.clamp(min=0) + torch.log1p(torch.exp(-u.abs())) - 0.69314718056
+        want = a.T @ dz[rows].double()
+        off = float((dw[t] - want).norm() / want.norm())
+        assert off < 7e-7
