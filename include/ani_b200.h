@@ -370,8 +370,8 @@ int ani_scale_by_loss_f32(float* grads, long long n, const float* l2s, int n_mol
  * element without rows are written as zeros where a pointer is given).  1 <= width <= 4096.  Strides count values, are at
  * least the width and need no alignment; rows that are 16-byte aligned are read faster.  Outputs are contiguous and written,
  * not added to.  Nothing is allocated: the calls with sums over rows take a workspace of the stated size, 16-byte aligned
- * (one per call in flight; its content does not matter; size 0: NULL will do).  All sums are formed in a fixed order, in the type of the rows:
- * results are bit-reproducible.
+ * (one per call in flight; its content does not matter; size 0: NULL will do).  All sums are formed in a fixed order, those over
+ * rows and columns in the type of the rows: results are bit-reproducible.
  *
  * Layer norm:  y = gain (x - mean) rstd + bias,  rstd = 1 / sqrt(variance + eps)  (variance: divided by the width).
  */
@@ -421,7 +421,9 @@ int ani_checkpoint_activation_grad_f32(const unsigned char* codes, const float* 
 
 /*
  * Weight gradient of the dense layer behind the activation:  grad_w[t] = sum over the rows of element t of
- * act(...)^T grad_z,  [width][out_width], the activations recomputed from the checkpoint; 1 <= out_width <= 4096.
+ * act(...)^T grad_z,  [width][out_width], the activations recomputed from the checkpoint; 1 <= out_width <= 4096.  Products in
+ * three tf32 parts with float32 sums, off by 2e-7 to 4e-7 in the 2-norm (split_precision of the networks does not choose here).
+ * What is not finite, in a row of the checkpoint or of grad_z, comes out as NaN.
  * workspace: ani_checkpoint_weight_grad_workspace_bytes(width, out_width, acs_host).
  */
 int ani_checkpoint_weight_grad_f32(const unsigned char* codes, const float* blocks, const float* mean, const float* rstd,

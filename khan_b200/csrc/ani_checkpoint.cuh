@@ -14,9 +14,9 @@
 //
 // One byte a value and 8 bytes a block (6 %) instead of the 8 bytes a value that z and a, or a and its derivative, take.
 //
-// 9.06 bytes a value either way.  110,000 x 512 with a norm: forward 86 us with celu, 93 with softplus (78 us of traffic; bound
-// by instructions, 40 for 32 values, 70 % of the issue slots), backward 90 and 96 us (bound by the latency of its loads: a row's
-// sums, xhat and gradients are 126 registers, which leaves 16 warps an SM).
+// 9.06 bytes a value either way.  110,000 x 512 with a norm, one call behind the other: forward 87 us with celu, 91 with softplus
+// (78 us of traffic; bound by instructions, 40 for 32 values, 70 % of the issue slots), backward with its sums 96 and 100 us (bound
+// by the latency of its loads: a row's sums, xhat and gradients are 126 registers, which leaves 16 warps an SM).
 #pragma once
 
 #include "ani_mlp.cuh"

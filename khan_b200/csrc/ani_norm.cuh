@@ -7,7 +7,7 @@
 //
 // A row belongs to a TEAM of threads (8, 16 or 32 lanes of a warp, or 2, 4 or 8 warps), which keeps it in registers: thread l
 // holds the NV groups of four consecutive columns 4 (l + k TEAM), so that the row is read once and the variance is the
-// two-pass one (a mean far from zero costs nothing).  Columns are four to a thread whether or not the rows are 16-byte
+// two-pass one (a mean far from zero costs the rounding of the mean itself, not that of its square).  Columns are four to a thread whether or not the rows are 16-byte
 // aligned; only the load instruction differs.  All sums are held in the type of the rows: 32 bits for float.
 //
 // Sums over rows: a CTA takes a contiguous range of rows of ONE element, its teams add up in registers, the CTA adds its
