@@ -8,7 +8,8 @@ dimension.  One launch covers all elements (two where sums over many rows are fo
 are bit-reproducible, nothing is kept from one call for the next, and a call can be captured into a CUDA graph.
 
 The functions are not recorded by autograd, but for :func:`layer_norm_autograd`; networks with checkpoints are differentiated
-by :class:`khan_b200.model.nn.MoleculeNN`.
+by :class:`khan_b200.model.nn.MoleculeNN`.  A backward pass is captured while no eager graph of the same parameters is alive:
+torch ties a parameter's gradient to the stream of the graph that it was first part of, and gives up in the capture.
 
 Rows may be strided (a slice of a wider tensor); other layouts are copied.  Widths go from 1 to 4096.  Layer norm takes
 float32 and float64, checkpoints float32.  There is no CPU path.
